@@ -46,7 +46,10 @@ setup(
             sources=sources,
             extra_compile_args={
                 "cxx": ["-O3", "-std=c++17"],
-                "nvcc": ["-O3", "-std=c++17"],
+                # no packed fp32 instructions: some of their forms have given
+                # wrong results on this hardware
+                "nvcc": ["-O3", "-std=c++17", "-Xclang", "-target-feature",
+                         "-Xclang", "-packed-fp32-ops"],
             },
             libraries=["hipblaslt"],
         )
