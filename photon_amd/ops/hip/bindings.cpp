@@ -57,6 +57,9 @@ torch::Tensor bias_grad(torch::Tensor dy);
 torch::Tensor fused_linear(torch::Tensor x, torch::Tensor w,
                            c10::optional<torch::Tensor> b);
 
+torch::Tensor embedding(torch::Tensor ids, torch::Tensor w, double scale,
+                        at::ScalarType out_dtype);
+
 }  // namespace photon_hip
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -90,6 +93,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "flash attention forward on packed [B,S,3HD] qkv");
   m.def("attn_bwd_qkv", &attn_bwd_qkv,
         "flash attention backward on packed qkv; returns dqkv");
+  m.def("embedding", &embedding,
+        "scaled embedding lookup with a sorted-token gradient");
   m.def("mfma_probe", &mfma_probe);
   m.def("pack_probe", &pack_probe);
 }

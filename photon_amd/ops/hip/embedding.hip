@@ -1,0 +1,570 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens (CDNA4).
+//
+//   forward:  y[n, :]  = round(scale * W[ids[n], :])
+//   backward: dW[v, :] = round(scale * sum over {n: ids[n] = v} of dy[n, :])
+//
+// Both only move memory. The gradient is a dense [V, D] tensor, so most of
+// what it writes are the zero rows of the tokens that did not occur.
+//
+// The sum is deterministic: positions are sorted by (token, position) with a
+// stable radix sort, every wave adds up the rows of CHUNK sorted positions,
+// and a token whose positions spread over several chunks is joined from the
+// chunks' partial rows in their order. Floating-point atomics would be
+// shorter, but their order changes from run to run, and the frequent tokens
+// of a text serialise on their rows. Sums are held in fp32 and rounded once.
+//
+// Ids outside [0, V) read as NaN rows and have no gradient.
+
+#include "host_common.h"
+
+
+namespace photon_hip {
+
+namespace {
+
+constexpr int EMB_BLOCK = 256;
+constexpr long MAX_GRID = 1L << 23;  // blocks; a grid has < 2^32 threads
+
+// VEC elements of a row, widened to fp32
+template <int VEC, typename T>
+DEV_INLINE void load_vec(const T* p, float* f) {
+  if constexpr (VEC == 1) {
+    f[0] = load_f32<T>(p, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) {
+      const floatx4 v = load4<T>(p + i);
+      f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
+    }
+  }
+}
+
+DEV_INLINE unsigned short round_bf16(float f) {
+  union { __bf16 b; unsigned short u; } r;
+  r.b = (__bf16)f;  // nearest even, NaN stays NaN
+  return r.u;
+}
+
+template <int VEC, typename T>
+DEV_INLINE void store_vec(T* p, const float* f) {
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (VEC == 1) {
+      p[0] = f[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; i += 4)
+        *reinterpret_cast<floatx4*>(p + i) =
+            floatx4{f[i], f[i + 1], f[i + 2], f[i + 3]};
+    }
+  } else {
+    if constexpr (VEC == 1) {
+      p[0] = round_bf16(f[0]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; i += 4) {
+        shortx4 r;
+        r.x = (short)round_bf16(f[i]);
+        r.y = (short)round_bf16(f[i + 1]);
+        r.z = (short)round_bf16(f[i + 2]);
+        r.w = (short)round_bf16(f[i + 3]);
+        *reinterpret_cast<shortx4*>(p + i) = r;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Forward: a block copies `rows` rows, a thread VEC columns at a time.
+// ---------------------------------------------------------------------------
+template <typename I, typename TW, typename TO, int VEC>
+__global__ __launch_bounds__(EMB_BLOCK) void embed_fwd_kernel(
+    const I* __restrict__ ids, const TW* __restrict__ w, long w_rs,
+    TO* __restrict__ out, long N, int D, long V, float scale, int rows) {
+  const int cpr = D / VEC;
+  for (long row0 = (long)blockIdx.x * rows; row0 < N;
+       row0 += (long)gridDim.x * rows) {
+    const int items = (int)min((long)rows, N - row0) * cpr;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < items; i += EMB_BLOCK) {
+      const int r = i / cpr;
+      const int c = (i - r * cpr) * VEC;
+      const long id = (long)ids[row0 + r];
+      float f[VEC];
+      if (id >= 0 && id < V) {
+        load_vec<VEC, TW>(w + id * w_rs + c, f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f[j] *= scale;
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f[j] = __builtin_nanf("");
+      }
+      store_vec<VEC, TO>(out + (row0 + r) * (long)D + c, f);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Backward, step 1: stable radix sort of (token, position), 8 bits a pass.
+//
+// A block owns `tile` consecutive items; counts[block][digit] of a pass are
+// made by the pass before (by a kernel of their own for the first one), and
+// every scatter block derives its places from all blocks' counts, which
+// stands for a scan kernel in between. At most SORT_BLOCKS blocks, so that
+// these counts stay at 128 KiB.
+// ---------------------------------------------------------------------------
+constexpr int SORT_BLOCKS = 128;
+constexpr int SORT_TILE = 1024;
+constexpr int DIGITS = 256;
+constexpr int SORT_WAVES = EMB_BLOCK / WAVE;
+
+template <typename I>
+DEV_INLINE unsigned token_key(const I* ids, long i, long V) {
+  const long id = (long)ids[i];
+  return (id >= 0 && id < V) ? (unsigned)id : (unsigned)V;  // sorted last
+}
+
+template <typename I>
+__global__ __launch_bounds__(EMB_BLOCK) void sort_count_kernel(
+    const I* __restrict__ ids, int N, long V, int tile,
+    unsigned* __restrict__ counts, int more_passes) {
+  __shared__ unsigned hist[DIGITS];
+  hist[threadIdx.x] = 0;
+  __syncthreads();
+  const long b0 = (long)blockIdx.x * tile;
+  const long b1 = min(b0 + tile, (long)N);
+  for (long i = b0 + threadIdx.x; i < b1; i += EMB_BLOCK)
+    atomicAdd(&hist[token_key(ids, i, V) & 255u], 1u);
+  __syncthreads();
+  const int at = blockIdx.x * DIGITS + threadIdx.x;
+  counts[at] = hist[threadIdx.x];
+  // the following passes' counts start at zero
+  const int stride = gridDim.x * DIGITS;
+  for (int p = 1; p <= more_passes; ++p) counts[p * stride + at] = 0;
+}
+
+template <typename I, bool FIRST>
+__global__ __launch_bounds__(EMB_BLOCK) void sort_scatter_kernel(
+    const I* __restrict__ ids, const unsigned* __restrict__ keys_in,
+    const unsigned* __restrict__ pos_in, unsigned* __restrict__ keys_out,
+    unsigned* __restrict__ pos_out, int N, long V, int tile, int shift,
+    const unsigned* __restrict__ counts, unsigned* __restrict__ next_counts) {
+  __shared__ unsigned offs[SORT_WAVES][DIGITS];
+  __shared__ unsigned totals[DIGITS];
+  const int tid = threadIdx.x;
+  const int lane = tid & (WAVE - 1);
+  const int wid = tid / WAVE;
+  const int nblk = gridDim.x;
+
+  // this thread's digit: items in earlier blocks, and in all blocks
+  unsigned before = 0, total = 0;
+#pragma unroll 16
+  for (int b = 0; b < nblk; ++b) {
+    const unsigned c = counts[b * DIGITS + tid];
+    total += c;
+    before += b < (int)blockIdx.x ? c : 0u;
+  }
+  totals[tid] = total;
+#pragma unroll
+  for (int w = 0; w < SORT_WAVES; ++w) offs[w][tid] = 0;
+  __syncthreads();
+  for (int d = 1; d < DIGITS; d <<= 1) {  // inclusive scan over the digits
+    const unsigned x = tid >= d ? totals[tid - d] : 0u;
+    __syncthreads();
+    totals[tid] += x;
+    __syncthreads();
+  }
+  const unsigned base = totals[tid] - total + before;
+
+  // a wave owns a quarter of the tile, in order
+  const int per_wave = tile / SORT_WAVES;
+  const long w0 = (long)blockIdx.x * tile + (long)wid * per_wave;
+  const long w1 = min(w0 + per_wave, (long)N);
+  for (long i = w0 + lane; i < w1; i += WAVE) {
+    const unsigned k = FIRST ? token_key(ids, i, V) : keys_in[i];
+    atomicAdd(&offs[wid][(k >> shift) & 255u], 1u);
+  }
+  __syncthreads();
+  unsigned run = base;
+#pragma unroll
+  for (int w = 0; w < SORT_WAVES; ++w) {
+    const unsigned c = offs[w][tid];
+    offs[w][tid] = run;
+    run += c;
+  }
+  __syncthreads();
+  volatile unsigned* mine = offs[wid];
+  for (long i0 = w0; i0 < w1; i0 += WAVE) {
+    const long i = i0 + lane;
+    const bool live = i < w1;
+    unsigned k = 0, pos = 0;
+    if (live) {
+      k = FIRST ? token_key(ids, i, V) : keys_in[i];
+      pos = FIRST ? (unsigned)i : pos_in[i];
+    }
+    const unsigned digit = (k >> shift) & 255u;
+    unsigned long long same = __ballot(live);
+#pragma unroll
+    for (int bit = 0; bit < 8; ++bit) {
+      const unsigned long long one = __ballot((digit >> bit) & 1u);
+      same &= ((digit >> bit) & 1u) ? one : ~one;
+    }
+    if (live) {
+      const int rank = __popcll(same & ((1ull << lane) - 1ull));
+      const unsigned at = mine[digit];
+      __builtin_amdgcn_wave_barrier();
+      if (rank == 0) mine[digit] = at + (unsigned)__popcll(same);
+      const unsigned dst = at + rank;
+      keys_out[dst] = k;
+      pos_out[dst] = pos;
+      if (next_counts)
+        atomicAdd(&next_counts[(dst / (unsigned)tile) * DIGITS +
+                               ((k >> (shift + 8)) & 255u)],
+                  1u);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Backward, step 2: sums over CHUNK sorted positions, COLS columns a wave.
+// A segment (one token's positions) inside its chunk is final; one that came
+// from the chunk before goes to head[chunk], one that goes on to the next
+// (and began here) to tail[chunk]. The blocks behind the sums' write the zero
+// rows: each lane looks its token up in the sorted keys.
+// ---------------------------------------------------------------------------
+constexpr int CHUNK = 32;
+constexpr int FILL_ROWS = 16;  // table rows a filling wave looks after
+
+template <typename TG, typename TW, int VEC>
+__global__ __launch_bounds__(EMB_BLOCK) void embed_sum_kernel(
+    const TG* __restrict__ dy, const unsigned* __restrict__ keys,
+    const unsigned* __restrict__ pos, TW* __restrict__ dw,
+    float* __restrict__ head, float* __restrict__ tail, int N, int D, long V,
+    float scale, int sum_blocks) {
+  constexpr int COLS = WAVE * VEC;
+  const int lane = threadIdx.x & (WAVE - 1);
+  const int wid = threadIdx.x / WAVE;
+  if ((int)blockIdx.x >= sum_blocks) {
+    const long r0 =
+        ((long)(blockIdx.x - sum_blocks) * SORT_WAVES + wid) * FILL_ROWS;
+    const long r = r0 + lane;
+    bool absent = false;
+    if (lane < FILL_ROWS && r < V) {
+      int lo = 0, hi = N;  // first sorted position with key >= r
+      while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (keys[mid] < (unsigned)r) lo = mid + 1; else hi = mid;
+      }
+      absent = lo == N || keys[lo] != (unsigned)r;
+    }
+    unsigned long long todo = __ballot(absent);
+    const float zero[VEC] = {};
+    while (todo) {
+      const int i = __ffsll(todo) - 1;
+      todo &= todo - 1;
+      for (int c = lane * VEC; c < D; c += COLS)
+        store_vec<VEC, TW>(dw + (r0 + i) * D + c, zero);
+    }
+    return;
+  }
+  const int tiles = (D + COLS - 1) / COLS;
+  const long item = (long)blockIdx.x * SORT_WAVES + wid;
+  const long chunk = item / tiles;
+  const int c = (int)(item - chunk * tiles) * COLS + lane * VEC;
+  const long first = chunk * CHUNK;
+  if (first >= N) return;
+  const int count = (int)min((long)CHUNK, N - first);
+  const bool in = c < D;
+  // lane i holds sorted position first + i; lane CHUNK looks one further
+  const long mine = first + lane;
+  const unsigned key = (lane <= count && mine < N) ? keys[mine] : 0xffffffffu;
+  const unsigned p = (lane < count) ? pos[mine] : 0u;
+  const unsigned last = first > 0 ? keys[first - 1] : 0xffffffffu;
+  bool from_before = (unsigned)__builtin_amdgcn_readlane(key, 0) == last;
+
+  float acc[VEC] = {};
+  constexpr int U = 8;  // rows in flight
+  for (int i0 = 0; i0 < count; i0 += U) {
+    float f[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned row = __builtin_amdgcn_readlane(p, i0 + u);
+      if (in) load_vec<VEC, TG>(dy + (long)row * D + c, f[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u;
+      if (i < count) {
+        const unsigned k = __builtin_amdgcn_readlane(key, i);
+        const unsigned next = __builtin_amdgcn_readlane(key, i + 1);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] += f[u][j];
+        const bool ends = i + 1 == count || next != k;
+        if (ends) {
+          const bool goes_on = i + 1 == count && next == k;
+          if (in && k < (unsigned)V) {
+            if (from_before) {
+              store_vec<VEC, float>(head + chunk * D + c, acc);
+            } else if (goes_on) {
+              store_vec<VEC, float>(tail + chunk * D + c, acc);
+            } else {
+#pragma unroll
+              for (int j = 0; j < VEC; ++j) acc[j] *= scale;
+              store_vec<VEC, TW>(dw + (long)k * D + c, acc);
+            }
+          }
+          from_before = false;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+        }
+      }
+    }
+  }
+}
+
+// Step 3: a token that leaves the chunk it began in is that chunk's tail and
+// the heads of the chunks up to the one that holds its last position. The
+// block's waves take every fourth of them and are added in order.
+template <typename TW, int VEC>
+__global__ __launch_bounds__(EMB_BLOCK) void embed_join_kernel(
+    const unsigned* __restrict__ keys, const float* __restrict__ head,
+    const float* __restrict__ tail, TW* __restrict__ dw, int N, int D, long V,
+    float scale) {
+  constexpr int COLS = WAVE * VEC;
+  __shared__ float sums[SORT_WAVES][COLS];
+  const int lane = threadIdx.x & (WAVE - 1);
+  const int wid = threadIdx.x / WAVE;
+  const long chunk = blockIdx.x;
+  const long first = chunk * CHUNK;
+  const long end = first + CHUNK;  // first position of the next chunk
+  if (end >= N) return;
+  const unsigned k = keys[end - 1];
+  if (keys[end] != k || k >= (unsigned)V) return;
+  if (first > 0 && keys[first] == k && keys[first - 1] == k) return;
+  long lo = end, hi = N;  // first position after the token's
+  while (lo < hi) {
+    const long mid = lo + (hi - lo) / 2;
+    if (keys[mid] <= k) lo = mid + 1; else hi = mid;
+  }
+  const long last = (lo - 1) / CHUNK;  // heads chunk + 1 .. last
+  for (int c0 = 0; c0 < D; c0 += COLS) {
+    const int c = c0 + lane * VEC;
+    float acc[VEC] = {};
+    if (c < D) {
+      if (wid == 0) load_vec<VEC, float>(tail + chunk * D + c, acc);
+#pragma unroll 4
+      for (long h = chunk + 1 + wid; h <= last; h += SORT_WAVES) {
+        float f[VEC];
+        load_vec<VEC, float>(head + h * D + c, f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] += f[j];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sums[wid][lane * VEC + j] = acc[j];
+    __syncthreads();
+    if (wid == 0 && c < D) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        float s = sums[0][lane * VEC + j];
+#pragma unroll
+        for (int w = 1; w < SORT_WAVES; ++w) s += sums[w][lane * VEC + j];
+        acc[j] = s * scale;
+      }
+      store_vec<VEC, TW>(dw + (long)k * D + c, acc);
+    }
+  }
+}
+
+bool aligned(const void* p, int bytes) { return ((uintptr_t)p % bytes) == 0; }
+
+}  // namespace
+
+#define DISPATCH_IDS(TENSOR, ...)                                        \
+  if ((TENSOR).scalar_type() == at::kLong) {                             \
+    using id_t = long;                                                   \
+    __VA_ARGS__;                                                         \
+  } else {                                                               \
+    using id_t = int;                                                    \
+    __VA_ARGS__;                                                         \
+  }
+
+// Two tensors' types at once; TORCH_CHECKed by embedding().
+#define DISPATCH_TWO(A, B, ...)                                          \
+  if ((A) == at::kBFloat16 && (B) == at::kBFloat16) {                    \
+    using a_t = unsigned short; using b_t = unsigned short;              \
+    __VA_ARGS__;                                                         \
+  } else if ((A) == at::kBFloat16) {                                     \
+    using a_t = unsigned short; using b_t = float;                       \
+    __VA_ARGS__;                                                         \
+  } else if ((B) == at::kBFloat16) {                                     \
+    using a_t = float; using b_t = unsigned short;                       \
+    __VA_ARGS__;                                                         \
+  } else {                                                               \
+    using a_t = float; using b_t = float;                                \
+    __VA_ARGS__;                                                         \
+  }
+
+torch::Tensor embedding_fwd(const torch::Tensor& ids_in,
+                            const torch::Tensor& w, double scale,
+                            at::ScalarType out_dtype) {
+  const c10::DeviceGuard guard(w.device());
+  auto ids = ids_in.contiguous();
+  const long N = ids.numel(), V = w.size(0);
+  const int D = (int)w.size(1);
+  auto sizes = ids.sizes().vec();
+  sizes.push_back(D);
+  auto out = torch::empty(sizes, w.options().dtype(out_dtype));
+  if (N == 0 || D == 0) return out;
+  const long rs = w.stride(0);
+  const bool wide = D % 4 == 0 && rs % 4 == 0 &&
+                    aligned(w.data_ptr(), 4 * (int)w.element_size());
+  const bool wider = wide && D % 8 == 0 && rs % 8 == 0 &&
+                     aligned(w.data_ptr(), 16);
+  // about four vectors a thread
+  const int vec = wider ? 8 : wide ? 4 : 1;
+  const int rows = std::max(1, 4 * EMB_BLOCK / std::max(1, D / vec));
+  const long blocks = std::min<long>((N + rows - 1) / rows, MAX_GRID);
+  DISPATCH_IDS(ids, DISPATCH_TWO(w.scalar_type(), out_dtype, {
+    auto kernel = vec == 8   ? embed_fwd_kernel<id_t, a_t, b_t, 8>
+                  : vec == 4 ? embed_fwd_kernel<id_t, a_t, b_t, 4>
+                             : embed_fwd_kernel<id_t, a_t, b_t, 1>;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(EMB_BLOCK), 0, cur_stream(),
+                       (const id_t*)ids.data_ptr(), (const a_t*)w.data_ptr(),
+                       rs, (b_t*)out.data_ptr(), N, D, V, (float)scale, rows);
+  }));
+  return out;
+}
+
+torch::Tensor embedding_bwd(const torch::Tensor& dy_in,
+                            const torch::Tensor& ids_in, long V, double scale,
+                            at::ScalarType w_dtype) {
+  const c10::DeviceGuard guard(dy_in.device());
+  auto dy = dy_in.contiguous();
+  auto ids = ids_in.contiguous();
+  const long N = ids.numel();
+  const int D = (int)dy.size(-1);
+  TORCH_CHECK(N < (1L << 31) - CHUNK, "embedding: too many ids for a gradient");
+  auto dw = torch::empty({V, (long)D}, dy.options().dtype(w_dtype));
+  if (V == 0 || D == 0) return dw;
+  if (N == 0) return dw.zero_();
+  int passes = 1;
+  while (passes < 4 && (V >> (8 * passes)) != 0) ++passes;
+  // tiles of at least SORT_TILE, at most SORT_BLOCKS of them
+  const long tiles = std::min<long>((N + SORT_TILE - 1) / SORT_TILE, SORT_BLOCKS);
+  const int tile =
+      (int)(((N + tiles - 1) / tiles + EMB_BLOCK - 1) / EMB_BLOCK * EMB_BLOCK);
+  const int nblk = (int)((N + tile - 1) / tile);
+  const long chunks = (N + CHUNK - 1) / CHUNK;
+
+  auto iopt = dy.options().dtype(at::kInt);
+  auto sorted = torch::empty({4, N}, iopt);  // two pairs of (key, position)
+  auto counts = torch::empty({passes, (long)nblk * DIGITS}, iopt);
+  auto parts = torch::empty({2, chunks, (long)D}, dy.options().dtype(at::kFloat));
+  unsigned* sp = (unsigned*)sorted.data_ptr();
+  unsigned* cp = (unsigned*)counts.data_ptr();
+  const auto stream = cur_stream();
+  int at_pair = 0;
+  DISPATCH_IDS(ids, {
+    const id_t* ip = (const id_t*)ids.data_ptr();
+    hipLaunchKernelGGL((sort_count_kernel<id_t>), dim3(nblk), dim3(EMB_BLOCK),
+                       0, stream, ip, (int)N, V, tile, cp, passes - 1);
+    for (int p = 0; p < passes; ++p) {
+      unsigned* in = sp + (long)(1 - at_pair) * 2 * N;
+      unsigned* to = sp + (long)at_pair * 2 * N;
+      unsigned* c = cp + (long)p * nblk * DIGITS;
+      unsigned* next = p + 1 < passes ? c + (long)nblk * DIGITS : nullptr;
+      if (p == 0)
+        hipLaunchKernelGGL((sort_scatter_kernel<id_t, true>), dim3(nblk),
+                           dim3(EMB_BLOCK), 0, stream, ip, in, in + N, to,
+                           to + N, (int)N, V, tile, 8 * p, c, next);
+      else
+        hipLaunchKernelGGL((sort_scatter_kernel<id_t, false>), dim3(nblk),
+                           dim3(EMB_BLOCK), 0, stream, ip, in, in + N, to,
+                           to + N, (int)N, V, tile, 8 * p, c, next);
+      at_pair = 1 - at_pair;
+    }
+  });
+  const unsigned* keys = sp + (long)(1 - at_pair) * 2 * N;
+  const unsigned* pos = keys + N;
+  float* head = parts.data_ptr<float>();
+  float* tail = head + chunks * D;
+  const bool wide = D % 4 == 0 && aligned(dy.data_ptr(), 4 * (int)dy.element_size());
+  const int cols = WAVE * (wide ? 4 : 1);
+  const long items = chunks * ((D + cols - 1) / cols);
+  const long sum_blocks = (items + SORT_WAVES - 1) / SORT_WAVES;
+  const long fill_rows = SORT_WAVES * FILL_ROWS;
+  const long grid = sum_blocks + (V + fill_rows - 1) / fill_rows;
+  TORCH_CHECK(grid < MAX_GRID && chunks < MAX_GRID,
+              "embedding: gradient too large");
+  DISPATCH_TWO(dy.scalar_type(), w_dtype, {
+    auto sum = wide ? embed_sum_kernel<a_t, b_t, 4> : embed_sum_kernel<a_t, b_t, 1>;
+    hipLaunchKernelGGL(sum, dim3(grid), dim3(EMB_BLOCK), 0, stream,
+                       (const a_t*)dy.data_ptr(), keys, pos,
+                       (b_t*)dw.data_ptr(), head, tail, (int)N, D, V,
+                       (float)scale, (int)sum_blocks);
+    auto join = wide ? embed_join_kernel<b_t, 4> : embed_join_kernel<b_t, 1>;
+    if (chunks > 1)
+      hipLaunchKernelGGL(join, dim3(chunks - 1), dim3(EMB_BLOCK), 0, stream,
+                         keys, head, tail, (b_t*)dw.data_ptr(), (int)N, D, V,
+                         (float)scale);
+  });
+  return dw;
+}
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+class EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
+ public:
+  static torch::Tensor forward(AutogradContext* ctx, torch::Tensor w,
+                               torch::Tensor ids, double scale,
+                               int64_t out_dtype) {
+    at::AutoDispatchBelowADInplaceOrView g;
+    ctx->save_for_backward({ids});
+    ctx->saved_data["rows"] = w.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["dtype"] = (int64_t)w.scalar_type();
+    return embedding_fwd(ids, w, scale, (at::ScalarType)out_dtype);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "embedding: a second derivative is not supported "
+                "(create_graph=True)");
+    auto ids = ctx->get_saved_variables()[0];
+    auto dw = embedding_bwd(grads[0], ids, ctx->saved_data["rows"].toInt(),
+                            ctx->saved_data["scale"].toDouble(),
+                            (at::ScalarType)ctx->saved_data["dtype"].toInt());
+    return {dw, torch::Tensor(), torch::Tensor(), torch::Tensor()};
+  }
+};
+
+bool known_dtype(at::ScalarType t) {
+  return t == at::kFloat || t == at::kBFloat16;
+}
+
+}  // namespace
+
+torch::Tensor embedding(torch::Tensor ids, torch::Tensor w, double scale,
+                        at::ScalarType out_dtype) {
+  TORCH_CHECK(w.dim() == 2 && w.is_cuda() && known_dtype(w.scalar_type()),
+              "embedding: the table must be a 2D fp32 or bf16 GPU tensor");
+  TORCH_CHECK(w.size(1) < (1L << 30) && w.size(0) < (1L << 31),
+              "embedding: table too large");
+  TORCH_CHECK(w.size(1) <= 1 || w.stride(1) == 1,
+              "embedding: a table row must be contiguous");
+  TORCH_CHECK(ids.device() == w.device(), "embedding: ids on ", ids.device(),
+              ", table on ", w.device());
+  TORCH_CHECK(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt,
+              "embedding: ids must be int64 or int32");
+  TORCH_CHECK(known_dtype(out_dtype), "embedding: output must be fp32 or bf16");
+  if (w.requires_grad() && at::GradMode::is_enabled())
+    return EmbeddingFn::apply(w, ids, scale, (int64_t)out_dtype);
+  return embedding_fwd(ids, w, scale, out_dtype);
+}
+
+}  // namespace photon_hip
