@@ -59,6 +59,9 @@ torch::Tensor fused_linear(torch::Tensor x, torch::Tensor w,
 
 torch::Tensor embedding(torch::Tensor ids, torch::Tensor w, double scale,
                         at::ScalarType out_dtype);
+std::vector<torch::Tensor> tensor_norms(std::vector<torch::Tensor> ts);
+std::vector<torch::Tensor> clip_grads(std::vector<torch::Tensor> gs,
+                                      double max_norm);
 
 }  // namespace photon_hip
 
@@ -95,6 +98,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "flash attention backward on packed qkv; returns dqkv");
   m.def("embedding", &embedding,
         "scaled embedding lookup with a sorted-token gradient");
+  m.def("tensor_norms", &tensor_norms,
+        "global and per-tensor L2 norms of many tensors");
+  m.def("clip_grads", &clip_grads,
+        "clip many tensors in place by their global norm");
   m.def("mfma_probe", &mfma_probe);
   m.def("pack_probe", &pack_probe);
 }

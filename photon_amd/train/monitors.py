@@ -17,6 +17,8 @@ from collections import deque
 
 import torch
 
+from ..ops.clip import tensor_norms
+
 MI355X_BF16_DENSE_PEAK = 2.5e15  # FLOP/s, dense (no sparsity)
 
 
@@ -97,26 +99,42 @@ class RuntimeEstimator:
 
 
 class OptimizerMonitor:
-    """L2 norm of the update moments (reference optimizer_monitor)."""
+    """L2 norms of the first moments and the gradients (reference
+    optimizer_monitor): the global ones, and with ``only_global`` False each
+    parameter's too. One sweep over all tensors and one wait for the device."""
 
-    def __init__(self, interval: int = 10):
-        self.interval = interval
+    def __init__(self, interval: int | str = 10, only_global: bool = True):
+        self.interval = (
+            int(interval.removesuffix("ba")) if isinstance(interval, str)
+            else int(interval)
+        )
+        self.only_global = only_global
 
     def batch_end(self, trainer, loss) -> dict:
         if trainer.timestamp.batch % self.interval != 0:
             return {}
-        sq_m, sq_g = 0.0, 0.0
+        moments, grads = {}, {}
+        names = {} if self.only_global else {
+            id(p): n for n, p in trainer.model.named_parameters()
+        }
         for group in trainer.optimizer.param_groups:
             for p in group["params"]:
                 st = trainer.optimizer.state.get(p)
+                name = names.get(id(p), str(len(grads)))
                 if st and "exp_avg" in st:
-                    sq_m += float(st["exp_avg"].float().pow(2).sum())
+                    moments[id(p)] = (name, st["exp_avg"])
                 if p.grad is not None:
-                    sq_g += float(p.grad.float().pow(2).sum())
-        return {
-            "optimizer/l2_norm_first_moment": sq_m**0.5,
-            "optimizer/l2_norm_grad": sq_g**0.5,
-        }
+                    grads[id(p)] = (name, p.grad)
+        out = {}
+        for key, found in (("optimizer/l2_norm_first_moment", moments),
+                           ("optimizer/l2_norm_grad", grads)):
+            total, each = tensor_norms([t for _, t in found.values()])
+            values = torch.cat([total.reshape(1), each]).tolist()
+            out[key] = values[0]
+            if not self.only_global:
+                out.update((f"{key}/{n}", v) for (n, _), v in
+                           zip(found.values(), values[1:]))
+        return out
 
 
 _MONITORS = {

@@ -35,6 +35,7 @@ sources = [
     str(HIP_DIR / "linear_lt.hip"),
     str(HIP_DIR / "bias_grad.hip"),
     str(HIP_DIR / "embedding.hip"),
+    str(HIP_DIR / "grad_norm.hip"),
     str(HIP_DIR / "fused_linear_fn.cpp"),
     str(HIP_DIR / "debug.hip"),
 ]
