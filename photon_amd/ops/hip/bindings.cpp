@@ -62,6 +62,11 @@ torch::Tensor embedding(torch::Tensor ids, torch::Tensor w, double scale,
 std::vector<torch::Tensor> tensor_norms(std::vector<torch::Tensor> ts);
 std::vector<torch::Tensor> clip_grads(std::vector<torch::Tensor> gs,
                                       double max_norm);
+torch::Tensor prefix_attention(torch::Tensor qkv, torch::Tensor prefix, long H,
+                               torch::Tensor slopes, torch::Tensor starts);
+torch::Tensor prefix_attention_decode(torch::Tensor qkv, torch::Tensor prefix,
+                                      long H, torch::Tensor slopes,
+                                      torch::Tensor cache, torch::Tensor held);
 
 }  // namespace photon_hip
 
@@ -102,6 +107,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "global and per-tensor L2 norms of many tensors");
   m.def("clip_grads", &clip_grads,
         "clip many tensors in place by their global norm");
+  m.def("prefix_attention", &prefix_attention,
+        "packed rows over a shared prefix and themselves (ALiBi)");
+  m.def("prefix_attention_decode", &prefix_attention_decode,
+        "one token per sequence over a shared prefix and a cache (ALiBi)");
   m.def("mfma_probe", &mfma_probe);
   m.def("pack_probe", &pack_probe);
 }

@@ -36,6 +36,7 @@ sources = [
     str(HIP_DIR / "bias_grad.hip"),
     str(HIP_DIR / "embedding.hip"),
     str(HIP_DIR / "grad_norm.hip"),
+    str(HIP_DIR / "prefix_attn.hip"),
     str(HIP_DIR / "fused_linear_fn.cpp"),
     str(HIP_DIR / "debug.hip"),
 ]
