@@ -71,11 +71,16 @@ def run_icl_eval(cfg, model, device) -> dict:
     from .eval import evaluate_icl_tasks, gauntlet_composite
 
     tok = load_tokenizer(icl_cfg.get("tokenizer_path"))
-    results = evaluate_icl_tasks(
-        model, tasks, tok, device=device,
-        max_seq_len=int(cfg["llm_config"].get("max_seq_len", 2048)),
-        limit_examples=icl_cfg.get("limit_examples"),
-    )
+    # fp32 weights on a GPU: the flash kernels take bf16
+    amp = (torch.device(device).type == "cuda"
+           and str(cfg["llm_config"].get("precision", "amp_bf16")) == "amp_bf16")
+    with torch.autocast("cuda", dtype=torch.bfloat16, enabled=amp):
+        results = evaluate_icl_tasks(
+            model, tasks, tok, device=device,
+            max_seq_len=int(cfg["llm_config"].get("max_seq_len", 2048)),
+            limit_examples=icl_cfg.get("limit_examples"),
+            share_prefix=bool(icl_cfg.get("share_prefix", False)),
+        )
     gauntlet = (cfg.get("eval_gauntlet_config") or {}).get("eval_gauntlet")
     results.update(gauntlet_composite(results, gauntlet))
     return results

@@ -33,6 +33,8 @@ from pathlib import Path
 import torch
 import torch.nn.functional as F
 
+from ..models.shared_prefix import SharedPrefix
+
 
 def _resolve_task_path(path: str | Path) -> Path:
     """Relative task paths resolve against the photon_amd package dir
@@ -83,10 +85,53 @@ def _continuation_stats(model, tok, context: str, continuation: str, device,
 
 
 @torch.no_grad()
+def _shared_stats(model, tok, pairs, device, max_len: int):
+    """_continuation_stats of several (context, continuation) pairs. The tokens
+    that all of them begin with (one question's answers share the question and
+    its examples) run through the model once."""
+    rows = []
+    for context, continuation in pairs:
+        cont = tok.encode(continuation)
+        ids = (tok.encode(context) + cont)[-max_len:]
+        rows.append((ids, min(len(cont), len(ids) - 1)))
+    live = [(ids, n) for ids, n in rows if n > 0]
+    # the token before the first scored one stays with its sequence: its
+    # output is a prediction that is scored
+    most = min((len(ids) - n - 1 for ids, n in live), default=0)
+    prefix = live[0][0][:most] if live else []
+    for ids, _ in live[1:]:
+        same = next((i for i, (a, b) in enumerate(zip(prefix, ids)) if a != b),
+                    len(prefix))
+        prefix = prefix[:same]
+    if len(live) < 2 or not prefix:
+        return [_continuation_stats(model, tok, c, a, device, max_len)
+                for c, a in pairs]
+    shared = SharedPrefix(model, prefix)
+    own = [ids[len(prefix):-1] for ids, _ in live]
+    hidden = shared.score(own)
+    stats, at = [], 0
+    scored = iter(own)
+    for ids, n in rows:
+        if n <= 0:
+            stats.append((0.0, 0, 0.0))
+            continue
+        at += len(next(scored))
+        logits = shared.logits(hidden[at - n:at])
+        tgt = torch.tensor(ids[-n:], dtype=torch.long, device=logits.device)
+        ce = float(F.cross_entropy(logits.float(), tgt, reduction="sum"))
+        stats.append((ce, n, int((logits.argmax(-1) == tgt).sum())))
+    return stats
+
+
+@torch.no_grad()
 def _greedy_generate(model, tok, prompt: str, device, max_len: int,
                      max_new_tokens: int = 24,
-                     stop_strings: list[str] | None = None) -> str:
+                     stop_strings: list[str] | None = None,
+                     share_prefix: bool = False) -> str:
     ids = tok.encode(prompt)[-(max_len - max_new_tokens):]
+    if share_prefix and ids:
+        return _generate_cached(model, tok, ids, max_new_tokens,
+                                stop_strings or [])
     x = torch.tensor([ids], dtype=torch.long, device=device)
     out_ids: list[int] = []
     for _ in range(max_new_tokens):
@@ -98,6 +143,24 @@ def _greedy_generate(model, tok, prompt: str, device, max_len: int,
         for stop in stop_strings or []:
             if stop in text:
                 return text.split(stop)[0]
+    return tok.decode(out_ids)
+
+
+def _generate_cached(model, tok, ids, max_new_tokens, stop_strings) -> str:
+    """Greedy generation that runs each token through the model once."""
+    shared = SharedPrefix(model, ids)
+    shared.begin(1, max_new_tokens)
+    hidden = shared.last_hidden
+    out_ids: list[int] = []
+    while len(out_ids) < max_new_tokens:
+        nxt = shared.logits(hidden)[-1].argmax().view(1)
+        out_ids.append(int(nxt))
+        text = tok.decode(out_ids)
+        for stop in stop_strings:
+            if stop in text:
+                return text.split(stop)[0]
+        if len(out_ids) < max_new_tokens:
+            hidden = shared.step(nxt)
     return tok.decode(out_ids)
 
 
@@ -131,10 +194,15 @@ def _fewshot_prefix(examples: list[dict], i: int, k: int, kind: str,
 @torch.no_grad()
 def evaluate_icl_tasks(model, tasks_cfg, tokenizer, device="cpu",
                        max_seq_len: int = 2048,
-                       limit_examples: int | None = None) -> dict[str, float]:
+                       limit_examples: int | None = None,
+                       share_prefix: bool = False) -> dict[str, float]:
     """Returns {"metrics/icl/{label}/accuracy": v, ...} per task; tasks
     whose dataset_uri is absent are skipped with a metric of nan (the
-    reference's remote datasets are not fetchable offline)."""
+    reference's remote datasets are not fetchable offline).
+
+    ``share_prefix``: the options of one example run as one batch over the
+    tokens they share, and generation keeps the keys and values of earlier
+    tokens (models/shared_prefix.py). The scores are the same up to rounding."""
     model.eval()
     results: dict[str, float] = {}
     for task in tasks_cfg or []:
@@ -162,6 +230,7 @@ def evaluate_icl_tasks(model, tasks_cfg, tokenizer, device="cpu",
             acc, cat_acc = _eval_task_once(
                 model, tokenizer, examples, kind, delim, prelim, cot, stops,
                 n_fewshot, do_norm, has_categories, device, max_seq_len,
+                share_prefix,
             )
             if shot_i == 0:
                 results[f"metrics/icl/{label}/accuracy"] = acc
@@ -176,7 +245,13 @@ def evaluate_icl_tasks(model, tasks_cfg, tokenizer, device="cpu",
 @torch.no_grad()
 def _eval_task_once(model, tokenizer, examples, kind, delim, prelim, cot,
                     stops, n_fewshot, do_norm, has_categories, device,
-                    max_seq_len):
+                    max_seq_len, share_prefix=False):
+    def option_stats(pairs):
+        if share_prefix:
+            return _shared_stats(model, tokenizer, pairs, device, max_seq_len)
+        return [_continuation_stats(model, tokenizer, c, a, device, max_seq_len)
+                for c, a in pairs]
+
     cat_correct: dict[str, float] = {}
     cat_total: dict[str, float] = {}
     if True:  # (kept indentation of the original loop body)
@@ -194,13 +269,9 @@ def _eval_task_once(model, tokenizer, examples, kind, delim, prelim, cot,
                 total += n
                 ex_correct, ex_total = c, n
             elif kind == "multiple_choice":
-                ces = []
-                for choice in ex["choices"]:
-                    ce, n, _ = _continuation_stats(
-                        model, tokenizer, shots + prelim + ex["query"] + delim,
-                        choice, device, max_seq_len,
-                    )
-                    ces.append(ce / max(n, 1))
+                context = shots + prelim + ex["query"] + delim
+                ces = [ce / max(n, 1) for ce, n, _ in option_stats(
+                    [(context, choice) for choice in ex["choices"]])]
                 ok_mc = int(min(range(len(ces)), key=ces.__getitem__)
                             == int(ex["gold"]))
                 correct += ok_mc
@@ -209,13 +280,9 @@ def _eval_task_once(model, tokenizer, examples, kind, delim, prelim, cot,
             elif kind == "schema":
                 # choose the context option that best explains the SAME
                 # continuation (winograd-style)
-                ces = []
-                for opt in ex["context_options"]:
-                    ce, n, _ = _continuation_stats(
-                        model, tokenizer, shots + opt + delim,
-                        ex["continuation"], device, max_seq_len,
-                    )
-                    ces.append(ce / max(n, 1))
+                ces = [ce / max(n, 1) for ce, n, _ in option_stats(
+                    [(shots + opt + delim, ex["continuation"])
+                     for opt in ex["context_options"]])]
                 ok_sc = int(min(range(len(ces)), key=ces.__getitem__)
                             == int(ex["gold"]))
                 correct += ok_sc
@@ -225,6 +292,7 @@ def _eval_task_once(model, tokenizer, examples, kind, delim, prelim, cot,
                 gen = _greedy_generate(
                     model, tokenizer, shots + prelim + ex["context"] + delim,
                     device, max_seq_len, stop_strings=stops,
+                    share_prefix=share_prefix,
                 )
                 if cot and cot in gen:
                     gen = gen.split(cot)[-1]

@@ -1,3 +1,4 @@
 from .mpt import MPTCausalLM, MPTConfig, build_model
+from .shared_prefix import SharedPrefix
 
-__all__ = ["MPTCausalLM", "MPTConfig", "build_model"]
+__all__ = ["MPTCausalLM", "MPTConfig", "SharedPrefix", "build_model"]

@@ -24,6 +24,7 @@ import torch.nn.functional as F
 
 from ..ops.attention import alibi_slopes, flash_attention, flash_attention_qkv
 from ..ops.cross_entropy import fused_cross_entropy
+from ..ops.embedding import FusedEmbedding
 from ..ops.layernorm import FusedLayerNorm
 from ..ops.linear import lt_available, lt_linear, lt_mlp
 
@@ -41,6 +42,8 @@ class MPTConfig:
     no_bias: bool = False
     init_std: float = 0.02
     loss_impl: str = "fused"  # "fused" (HIP CE kernel) | "torch"
+    emb_scale: float = 1.0  # token embeddings are multiplied by this
+    emb_impl: str = "fused"  # "fused" (HIP lookup and gradient) | "torch"
 
     @property
     def d_head(self) -> int:
@@ -58,6 +61,8 @@ class MPTConfig:
             vocab_size=int(model_cfg.get("vocab_size", 50368)),
             attn_impl=str(attn.get("attn_impl", "flash")),
             no_bias=bool(model_cfg.get("no_bias", False)),
+            emb_scale=float(model_cfg.get("emb_scale", 1.0)),
+            emb_impl=str(model_cfg.get("emb_impl", "fused")),
         )
 
 
@@ -81,9 +86,10 @@ class MPTAttention(nn.Module):
         slopes = alibi_slopes(cfg.n_heads, cfg.alibi_bias_max)
         self.register_buffer("slopes", slopes, persistent=False)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        B, S, D = x.shape
-        H, dh = self.n_heads, self.d_head
+    def forward(self, x: torch.Tensor, attend=None) -> torch.Tensor:
+        """``attend(qkv, n_heads, slopes, impl)``, if given, stands for the
+        causal attention over the packed Wqkv output [B, S, 3*H*dh]."""
+        H = self.n_heads
         # Fused-linear path (C++ autograd + HIP bias-grad backward). Only
         # for PLAIN nn.Linear projections: tensor-parallel swaps replace
         # them with Column/RowParallelLinear whose forward carries the TP
@@ -102,9 +108,12 @@ class MPTAttention(nn.Module):
         # Packed path: the HIP kernels read [B,S,3,H,dh] strided directly
         # (no chunk/transpose/contiguous copies); falls back to reshape +
         # SDPA on CPU / attn_impl=torch.
-        out = flash_attention_qkv(
-            qkv, H, self.slopes, causal=True, impl=self.cfg.attn_impl
-        )  # [B, S, H*dh]
+        if attend is not None:
+            out = attend(qkv, H, self.slopes, self.cfg.attn_impl)
+        else:
+            out = flash_attention_qkv(
+                qkv, H, self.slopes, causal=True, impl=self.cfg.attn_impl
+            )  # [B, S, H*dh]
         if fused:
             return lt_linear(out, self.out_proj.weight, self.out_proj.bias)
         return self.out_proj(out)
@@ -139,7 +148,8 @@ class MPTBlock(nn.Module):
         self.norm_2 = FusedLayerNorm(cfg.d_model, bias=bias)
         self.ffn = MPTMLP(cfg)
 
-    def forward(self, x: torch.Tensor, pending: torch.Tensor | None = None):
+    def forward(self, x: torch.Tensor, pending: torch.Tensor | None = None,
+                attend=None):
         """Residual-add/LN fusion flow: ``pending`` is the PREVIOUS
         block's un-added FFN output (or None for block 0); the add rides
         the norm_1 kernel. Returns (residual_stream, ffn_out) — the caller
@@ -150,7 +160,7 @@ class MPTBlock(nn.Module):
             x, n1 = self.norm_1.forward_add(x, pending)
         else:
             n1 = self.norm_1(x)
-        a = self.attn(n1)
+        a = self.attn(n1, attend)
         x, n2 = self.norm_2.forward_add(x, a)
         return x, self.ffn(n2)
 
@@ -161,23 +171,22 @@ class MPTModel(nn.Module):
 
     def __init__(self, cfg: MPTConfig):
         super().__init__()
-        self.wte = nn.Embedding(cfg.vocab_size, cfg.d_model)
+        self.wte = FusedEmbedding(cfg.vocab_size, cfg.d_model,
+                                  scale=cfg.emb_scale, impl=cfg.emb_impl)
         self.blocks = nn.ModuleList(MPTBlock(cfg) for _ in range(cfg.n_layers))
         self.norm_f = FusedLayerNorm(cfg.d_model, bias=not cfg.no_bias)
 
-    def forward(self, input_ids: torch.Tensor) -> torch.Tensor:
+    def forward(self, input_ids: torch.Tensor, attends=None) -> torch.Tensor:
+        """``attends``: one callable for each block (MPTAttention.forward)."""
+        # wte writes the autocast compute dtype (bf16) itself, so the residual
+        # stream is bf16: in fp32 every LayerNorm / residual add / attention
+        # input would move twice the bytes (measured 16.6% of step time in
+        # fp32 LN alone, profiles/r01). Statistics inside the LN/CE kernels
+        # still accumulate in fp32.
         x = self.wte(input_ids)
-        # Keep the residual stream in the autocast compute dtype (bf16):
-        # nn.Embedding outputs fp32 under autocast, and without this cast
-        # every LayerNorm / residual add / attention input runs fp32 —
-        # doubling HBM traffic on a bandwidth-bound chip (measured 16.6% of
-        # step time in fp32 LN alone, profiles/r01). Statistics inside the
-        # LN/CE kernels still accumulate in fp32.
-        if torch.is_autocast_enabled(x.device.type):
-            x = x.to(torch.get_autocast_dtype(x.device.type))
         pending = None
-        for block in self.blocks:
-            x, pending = block(x, pending)
+        for i, block in enumerate(self.blocks):
+            x, pending = block(x, pending, attends[i] if attends else None)
         # final residual add fused into norm_f
         _, y = self.norm_f.forward_add(x, pending)
         return y
@@ -243,8 +252,9 @@ def resize_vocab(model: MPTCausalLM, new_vocab: int) -> MPTCausalLM:
     old = model.transformer.wte
     if new_vocab == old.num_embeddings:
         return model
-    new = nn.Embedding(new_vocab, old.embedding_dim,
-                       device=old.weight.device, dtype=old.weight.dtype)
+    new = FusedEmbedding(new_vocab, old.embedding_dim, scale=old.scale,
+                         impl=old.impl, device=old.weight.device,
+                         dtype=old.weight.dtype)
     nn.init.normal_(new.weight, mean=0.0, std=model.cfg.init_std)
     keep = min(new_vocab, old.num_embeddings)
     new.weight.data[:keep] = old.weight.data[:keep]

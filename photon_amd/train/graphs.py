@@ -17,6 +17,8 @@ Contract:
   path pads nothing and always ticks full microbatches;
 * gradients ACCUMULATE into the captured .grad tensors — callers must zero
   with ``set_to_none=False`` (zero_()), never free them;
+* no loss of an earlier eager pass over the same parameters is alive when the
+  first microbatch is captured;
 * the optimizer step and scheduler run OUTSIDE the graph (dynamic lr);
 * weight VALUES may change between replays (the fed round copies new
   globals into the same parameter tensors — graph-safe).
@@ -51,6 +53,9 @@ class GraphedMicrobatch:
                     out = self.model(self.static_ids, labels=self.static_ids)
                     loss = out["loss"] / self.loss_div
                     loss.backward()
+        # A live eager graph keeps the leaves' accumulation nodes on the
+        # warm-up's stream, and a captured backward must not wait for that one.
+        del out, loss
         torch.cuda.current_stream().wait_stream(s)
         self._zero_grads()
         g = torch.cuda.CUDAGraph()

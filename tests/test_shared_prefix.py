@@ -1,0 +1,264 @@
+"""The model over a shared prefix, the ICL harness on it, and a training step
+that runs lookup, gradient and clipping together before the model is scored.
+
+Tolerances: on the CPU everything is fp32 and the two paths add the same
+numbers in another order: below 100 keys * 2^-24 for a softmax, a few of those
+a layer, values of unit size: 1e-4 for logits. Under autocast on the GPU each
+of about 8 roundings a layer moves a hidden state by up to 2^-8 of itself;
+with logits of std 0.3 (0.02 * sqrt(256) unit hidden values) that is 0.03 *
+0.3 rms over two layers, and 0.1 is ten times that.
+"""
+
+import copy
+import json
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from photon_amd.data.convert import ByteTokenizer
+from photon_amd.eval import evaluate_icl_tasks
+from photon_amd.eval.icl import _continuation_stats, _greedy_generate, _shared_stats
+from photon_amd.models import MPTCausalLM, MPTConfig, SharedPrefix
+from photon_amd.ops.clip import clip_grad_norm_
+
+gpu = pytest.mark.gpu
+
+
+def tiny(impl="torch", d=64, heads=2, layers=2, vocab=300, **kw):
+    torch.manual_seed(3)
+    return MPTCausalLM(MPTConfig(d_model=d, n_heads=heads, n_layers=layers, max_seq_len=128,
+                                 vocab_size=vocab, attn_impl=impl, **kw)).eval()
+
+
+def assert_scores(model, prefix, seqs, tol):
+    shared = SharedPrefix(model, prefix)
+    got = shared.logits(shared.score(seqs)).float()
+    dev, at = got.device, 0
+    with torch.no_grad():
+        for s in seqs:
+            if not s:
+                continue
+            whole = model(torch.tensor([prefix + s], device=dev))["logits"][0].float()
+            assert (got[at:at + len(s)] - whole[len(prefix):]).abs().max() < tol
+            at += len(s)
+        last = shared.logits(shared.last_hidden)[0].float()
+        whole = model(torch.tensor([prefix], device=dev))["logits"][0, -1].float()
+        assert (last - whole).abs().max() < tol
+        # the same tokens one by one: the sequences' common number of steps
+        live = [s for s in seqs if s]
+        steps = min(map(len, live))
+        shared.begin(len(live), steps)
+        for i in range(steps):
+            out = shared.logits(shared.step(torch.tensor([s[i] for s in live], device=dev))).float()
+            for row, s in zip(out, live):
+                ref = model(torch.tensor([prefix + s[:i + 1]], device=dev))["logits"][0, -1].float()
+                assert (row - ref).abs().max() < tol
+        with pytest.raises(IndexError, match="slots"):
+            shared.step(torch.zeros(len(live), dtype=torch.long))
+
+
+SEQS = [[5, 9, 200, 1], [7, 8], [], [1, 2, 3, 4, 5, 6, 7]]
+
+
+@pytest.mark.parametrize("scale", [1.0, 4.0])
+def test_scores_match_whole_sequences(scale):
+    assert_scores(tiny(emb_scale=scale), [11, 250, 3, 99, 42], SEQS, 1e-4)
+
+
+def test_shared_prefix_refusals():
+    m = tiny()
+    for bad in ([], [[1, 2]]):
+        with pytest.raises(ValueError, match="prefix_ids"):
+            SharedPrefix(m, bad)
+    with pytest.raises(TypeError, match="MPTCausalLM"):
+        SharedPrefix(torch.nn.Sequential(m), [1])
+    s = SharedPrefix(m, [1])
+    with pytest.raises(RuntimeError, match="begin"):
+        s.step(torch.tensor([1]))
+    with pytest.raises(ValueError, match="count and slots"):
+        s.begin(0, 4)
+    s.begin(2, 4)
+    with pytest.raises(ValueError, match="2 tokens"):
+        s.step(torch.tensor([1]))
+    assert s.score([[], []]).shape == (0, 64)
+
+
+def test_prefix_takes_no_gradient():
+    m = tiny()
+    s = SharedPrefix(m, [1, 2])
+    assert not s.score([[3]]).requires_grad and not s.last_hidden.requires_grad
+    s.begin(1, 1)
+    assert not s.step(torch.tensor([3])).requires_grad
+
+
+PAIRS = [
+    [("the sky is ", "blue"), ("the sky is ", "green and"), ("the sky is ", "b")],
+    [("a cat sat ", "down"), ("a cow sat ", "down")],  # contexts differ
+    [("xy", "z"), ("ab", "z")],  # nothing shared
+    [("only one ", "here")],
+    [("same ", ""), ("same ", "thing"), ("same ", "thin")],  # nothing to score
+    [("", "abc"), ("", "abd")],  # no context
+    [("long context " * 20, "one"), ("long context " * 20, "three")],  # cut off
+]
+
+
+@pytest.mark.parametrize("pairs", PAIRS)
+def test_shared_stats_match_single_ones(pairs):
+    m, tok = tiny(), ByteTokenizer()
+    want = [_continuation_stats(m, tok, c, a, "cpu", 100) for c, a in pairs]
+    got = _shared_stats(m, tok, pairs, "cpu", 100)
+    for (ce, n, ok), (ce2, n2, ok2) in zip(want, got):
+        assert n == n2 and ok == ok2 and abs(ce - ce2) <= 1e-4 * max(n, 1)
+
+
+@pytest.mark.parametrize("stops", [[], ["a"], ["\n"]])
+def test_cached_generation_matches(stops):
+    m, tok = tiny(), ByteTokenizer()
+    for prompt in ("tell me", "x", ""):
+        if not prompt:
+            continue
+        a = _greedy_generate(m, tok, prompt, "cpu", 100, 9, stops)
+        b = _greedy_generate(m, tok, prompt, "cpu", 100, 9, stops, share_prefix=True)
+        assert a == b
+
+
+def write_tasks(tmp_path):
+    rows = {
+        "multiple_choice": [{"query": f"question {i}", "choices": ["a", "bb", "c c"], "gold": i % 3} for i in range(4)],
+        "schema": [{"context_options": ["the cat", "the dog"], "continuation": f"ran {i}", "gold": 0} for i in range(3)],
+        "generation_task_with_answers": [{"context": f"who {i}", "answer": "me", "aliases": []} for i in range(2)],
+        "language_modeling": [{"context": "one two", "continuation": "three"}] * 2,
+    }
+    tasks = []
+    for kind, exs in rows.items():
+        f = tmp_path / f"{kind}.jsonl"
+        f.write_text("".join(json.dumps(e) + "\n" for e in exs))
+        tasks.append({"label": kind, "dataset_uri": str(f), "icl_task_type": kind, "num_fewshot": [0, 2]})
+    return tasks
+
+
+def test_icl_tasks_score_the_same(tmp_path):
+    tasks = write_tasks(tmp_path)
+    a = evaluate_icl_tasks(tiny(), tasks, ByteTokenizer(), max_seq_len=128)
+    b = evaluate_icl_tasks(tiny(), tasks, ByteTokenizer(), max_seq_len=128, share_prefix=True)
+    assert a == b and len(a) == 12
+
+
+def test_emb_scale_in_the_model():
+    """emb_scale is read from the configuration, survives a resize, and 1.0
+    leaves the model as it was."""
+    from photon_amd.models.mpt import build_model, resize_vocab
+
+    cfg = {"model": {"d_model": 64, "n_heads": 2, "n_layers": 1, "vocab_size": 50, "emb_scale": 8.0,
+                     "attn_config": {"attn_impl": "torch"}}}
+    torch.manual_seed(0)
+    m = build_model(cfg)
+    torch.manual_seed(0)
+    plain = build_model({"model": {**cfg["model"], "emb_scale": 1.0}})
+    assert all(torch.equal(a, b) for a, b in zip(m.parameters(), plain.parameters()))
+    ids = torch.randint(0, 50, (2, 5))
+    assert torch.equal(m.transformer.wte(ids), plain.transformer.wte(ids) * 8.0)
+    assert torch.equal(plain.transformer.wte(ids), F.embedding(ids, plain.transformer.wte.weight))
+    resize_vocab(m, 70)
+    assert m.transformer.wte.scale == 8.0 and m.transformer.wte(ids).shape == (2, 5, 64)
+
+
+# -- GPU --------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    return torch.device("cuda:0")
+
+
+@gpu
+@pytest.mark.parametrize("d,heads", [(256, 4), (256, 2)])
+@pytest.mark.parametrize("weights", ["autocast", "bf16"])
+def test_gpu_scores_match_whole_sequences(dev, d, heads, weights):
+    m = tiny("flash", d, heads).to(dev)
+    prefix = [(37 * i) % 300 for i in range(90)]
+    if weights == "bf16":
+        assert_scores(m.to(torch.bfloat16), prefix, SEQS, 0.1)
+    else:
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            assert_scores(m, prefix, SEQS, 0.1)
+
+
+@gpu
+def test_gpu_icl_tasks(dev, tmp_path):
+    m = tiny("flash", 256, 4).to(dev)
+    tok = ByteTokenizer()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        for pairs in PAIRS:
+            want = [_continuation_stats(m, tok, c, a, dev, 100) for c, a in pairs]
+            for (ce, n, _), (ce2, n2, _) in zip(want, _shared_stats(m, tok, pairs, dev, 100)):
+                assert n == n2 and abs(ce - ce2) <= 0.1 * max(n, 1)
+        got = evaluate_icl_tasks(m, write_tasks(tmp_path), tok, device=dev, max_seq_len=128, share_prefix=True)
+    assert len(got) == 12 and all(0.0 <= v <= 1.0 for v in got.values())
+
+
+@gpu
+def test_train_clip_then_score(dev):
+    """Two steps with the fused lookup, its gradient and clipping against the
+    same with torch's lookup and a loop over the gradients, then both models
+    score over a shared prefix."""
+    from photon_amd.ops.optim import DecoupledAdamW
+
+    ids = torch.randint(0, 300, (4, 64), device=dev)
+    models = [tiny("flash", 256, 4, emb_scale=4.0, emb_impl=i).train().to(dev) for i in ("fused", "torch")]
+    opts = [DecoupledAdamW(m.parameters(), lr=1e-3) for m in models]
+    for step in range(2):
+        norms = []
+        for m, opt in zip(models, opts):
+            opt.zero_grad()
+            with torch.autocast("cuda", dtype=torch.bfloat16):
+                m(ids, labels=ids)["loss"].backward()
+            ps = list(m.parameters())
+            if m.cfg.emb_impl == "fused":
+                want = math.sqrt(sum(float(p.grad.double().square().sum()) for p in ps))
+                total = float(clip_grad_norm_(ps, 0.1))
+                assert abs(total - want) <= 2.0**-22 * want
+            else:
+                total = math.sqrt(sum(float(p.grad.double().square().sum()) for p in ps))
+                for p in ps:
+                    p.grad.mul_(min(1.0, 0.1 / (total + 1e-6)))
+            norms.append(total)
+            opt.step()
+        if step == 0:
+            # one forward and backward with the same roundings; the embedding's
+            # gradient differs by fp32 sums of 256 terms
+            assert abs(norms[0] - norms[1]) <= 1e-4 * norms[1]
+            a, b = (m.transformer.wte.weight.grad for m in models)
+            assert (a - b).norm() <= 1e-4 * b.norm()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        a, b = (SharedPrefix(m.eval(), list(range(50))) for m in models)
+        x, y = (s.logits(s.score(SEQS)).float() for s in (a, b))
+    assert x.isfinite().all() and (x - y).abs().max() < 0.1
+
+
+@gpu
+def test_graphed_microbatch_matches_eager(dev):
+    """Lookup and gradient inside the captured training microbatch. Should a
+    library product choose another split in a graph, a bf16 value rounds to
+    its other neighbour: 2^-7 of some values, below 2^-8 in the norm."""
+    from photon_amd.train.graphs import GraphedMicrobatch
+
+    def amp():
+        return torch.autocast("cuda", dtype=torch.bfloat16)
+
+    eager, graphed = (tiny("flash", 256, 4, emb_scale=2.0).train().to(dev) for _ in range(2))
+    g = GraphedMicrobatch(graphed, amp, 1.0, 2, 64, dev)
+    for i in range(4):
+        ids = torch.randint(0, 300, (2, 64), device=dev)
+        if i:
+            g._zero_grads()
+        loss = float(g.run(ids))
+        eager.zero_grad()
+        with amp():
+            want = eager(ids, labels=ids)["loss"]
+            want.backward()
+        assert abs(loss - float(want.detach())) <= 2.0**-8 * loss
+        for a, b in zip(graphed.parameters(), eager.parameters()):
+            assert (a.grad - b.grad).norm() <= 2.0**-8 * b.grad.norm()
