@@ -1,0 +1,572 @@
+// Attention of a batch of sequences that share a long prefix (ALiBi, CDNA4).
+//
+// Sequence b continues the same P tokens with its own ones. Its query at own
+// position i (position P + i of the text) sees all P keys of the prefix and
+// its own keys 0..i:
+//
+//   w = q . k / sqrt(d) - slope_h * (P + i - pos_k),  o = softmax(w) v
+//
+// The prefix is the same for every row of every sequence, so the rows of all
+// sequences are stacked into the query tiles of ONE attention over it: a key
+// tile is read once for 32 * NW rows, whatever sequence they belong to, where
+// attention per sequence would read the prefix once per sequence. Behind the
+// prefix come the packed rows themselves, masked to a block diagonal.
+//
+// The key axis can be split over workgroups: each leaves (m, l, o) with
+// m = max w, l = sum e^(w - m), o = sum e^(w - m) v, and
+//   M = max m_i,  o = sum e^(m_i - M) o_i / sum e^(m_i - M) l_i
+// joins them. Statistics and sums are fp32; the probabilities are rounded to
+// bf16 for the second matrix product, as the values they weigh are.
+
+#pragma once
+
+#include "attn_kernels.h"
+
+namespace photon_hip {
+
+constexpr int PKB = 64;  // keys a tile
+
+// Buffer descriptor of `bytes` from `base` as four words (flags: a valid
+// format, see make_rsrc), and a copy of 16 bytes a lane to LDS through it.
+//
+// The builtin for this copy makes the compiler wait for ALL copies in flight
+// before a transposing LDS read, which it takes for a possible reader of the
+// tile that is still on its way: a stall of a memory latency every tile. The
+// copies written here are invisible to it and waited for by vm_wait0(). They
+// write no register; the wait states stand between a descriptor word that a
+// vector instruction wrote and its use.
+typedef __attribute__((ext_vector_type(4))) unsigned desc_t;
+DEV_INLINE desc_t make_desc(const __bf16* base, long bytes) {
+  const unsigned long a = (unsigned long)base;
+  return desc_t{(unsigned)a, (unsigned)(a >> 32) & 0xffffu, (unsigned)bytes,
+                0x27FACu};
+}
+DEV_INLINE unsigned lds_base(const char* smem) {
+  typedef __attribute__((address_space(3))) const char* lds_cp;
+  return __builtin_amdgcn_readfirstlane((unsigned)(size_t)(lds_cp)smem);
+}
+DEV_INLINE void copy16_to_lds(desc_t desc, unsigned lds, int offset) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 4\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds"
+      :
+      : "s"(lds), "v"(offset), "s"(desc)
+      : "memory", "m0");
+}
+
+// The larger of a row's two halves (lanes l and l + 32); NaN if one is.
+DEV_INLINE float swap_max(float x) {
+  union { float f; unsigned u; } a, b;
+  a.f = x;
+  const auto r = __builtin_amdgcn_permlane32_swap(a.u, a.u, false, false);
+  a.u = r[0];
+  b.u = r[1];
+  return __builtin_elementwise_maximum(a.f, b.f);
+}
+
+// Eight weights (rows of the score tile) as a fragment of the next product,
+// see pack_bfrag; the compiler places the conversions.
+DEV_INLINE bf16x8 pack_weights(const float* p) {
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+  union { bf16x2 v; unsigned u; } d[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    d[i].v[0] = (__bf16)p[2 * i];
+    d[i].v[1] = (__bf16)p[2 * i + 1];
+  }
+  const auto a = __builtin_amdgcn_permlane32_swap(d[0].u, d[2].u, false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap(d[1].u, d[3].u, false, false);
+  union { unsigned u[4]; bf16x8 v; } out;
+  out.u[0] = a[0];
+  out.u[1] = b[0];
+  out.u[2] = a[1];
+  out.u[3] = b[1];
+  return out.v;
+}
+
+// LDS: two buffers of a key and a value image (or, at the end, the fp32 rows
+// of all waves), and a word for each wave.
+constexpr int lds_images(int D, int nw) {
+  const int images = 4 * PKB * D * 2, rows = nw * 32 * D * 4;
+  return images > rows ? images : rows;
+}
+constexpr int lds_bytes(int D, int nw) { return lds_images(D, nw) + 64; }
+
+// Swapped product (keys x queries): lane holds query lane & 31, its 16
+// registers the keys (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5) of 32.
+//
+// `info` is each row's first own row (packed form) or, in the decode form, how
+// many own keys the row's sequence holds; there the kernel covers the prefix
+// only.
+template <int D, int NW, bool DECODE>
+__global__ __launch_bounds__(64 * NW, 2) void prefix_attn_kernel(
+    const __bf16* __restrict__ qkv, long q_rs, const __bf16* __restrict__ pk,
+    const __bf16* __restrict__ pv, long p_rs,
+    const float* __restrict__ slopes, const int* __restrict__ info,
+    __bf16* __restrict__ out, float* __restrict__ part_o,
+    float* __restrict__ part_ml, int T, int P, int H, int full, int splits) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int IMG = PKB * D * 2;  // bytes of a [64][D] image
+  constexpr bool D64 = D == 64;
+
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int hi = lane >> 5;
+  const int lq = lane & 31;
+  // the first `full` items (query tile, head) are whole, the others split
+  int item = blockIdx.x, split = 0, parts = 1;
+  if (item >= full) {
+    split = (item - full) % splits;
+    item = full + (item - full) / splits;
+    parts = splits;
+  }
+  const int h = item % H;
+  const int q0_block = item / H * (NW * QB);
+  const int my_q = q0_block + wave * QB + lq;
+  const int row = min(my_q, T - 1);
+
+  const float scale2 = rsqrtf((float)D) * LOG2E;
+  const float slope2 = slopes[h] * LOG2E;
+
+  const __bf16* q = qkv + (long)h * D;
+  const __bf16* k = q + (long)H * D;
+  const __bf16* v = k + (long)H * D;
+  pk += (long)h * D;
+  pv += (long)h * D;
+
+  bf16x8 qfrag[D / 16];
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk)
+    qfrag[kk] = *(const bf16x8*)(q + row * q_rs + kk * 16 + 8 * hi);
+
+  // own position of this lane's row, and the first packed row it may see
+  int first = 0, own = 0;
+  if (DECODE) {
+    own = max(info[row], 0);
+  } else {
+    first = min(max(info[row], 0), row);
+    own = row - first;
+  }
+
+  // key tiles: the prefix's, then the packed rows lo..hi_row of this block
+  const int n_pre = (P + PKB - 1) / PKB;
+  int lo = 0, n_own = 0, end_row = 0;
+  if (!DECODE) {
+    lo = __builtin_amdgcn_readfirstlane(
+        min(max(info[q0_block], 0), q0_block));
+    end_row = min(q0_block + NW * QB, T);
+    n_own = (end_row - lo + PKB - 1) / PKB;
+  }
+  const int n_all = n_pre + n_own;
+  const int t0 = (int)((long)n_all * split / parts);
+  const int t1 = (int)((long)n_all * (split + 1) / parts);
+
+  float m_run = -1e30f;  // finite: exp2(-huge) == 0 and no NaN from inf - inf
+  float l_run = 0.f;      // this half's share of the sum
+  f32x16 o_acc[D / 32];
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) o_acc[db] = f32x16{};
+
+  // The accumulators of the scores begin at slope * sqrt(d) * (key within the
+  // subtile); the rest of the bias is a constant of row and subtile that joins
+  // the maximum's subtraction.
+  f32x16 alibi;
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    alibi[r] = slopes[h] * sqrtf((float)D) *
+               (float)((r & 3) + 8 * (r >> 2) + 4 * hi);
+
+  // Staging: a wave-instruction moves 1 KiB to LDS, lane by lane in order;
+  // the swizzle is applied to the source. The descriptor starts at the tile
+  // (64-bit base), so a prefix of any length keeps 32-bit offsets, and ends
+  // with its last row: what lies behind reads as zeros.
+  constexpr int NWIN = IMG / 1024 / NW;
+  int dma_row[NWIN], dma_col[NWIN];
+#pragma unroll
+  for (int i = 0; i < NWIN; ++i) {
+    const int dest = (wave * NWIN + i) * 1024 + lane * 16;
+    const int r = dest / (D * 2);
+    dma_row[i] = r;
+    dma_col[i] =
+        (dest ^ (int)(swz_field((unsigned)r & 15u, D64) << 4)) % (D * 2);
+  }
+  const unsigned wave_win =
+      lds_base(smem) + __builtin_amdgcn_readfirstlane(wave) * (NWIN * 1024);
+  auto stage = [&](int t, int b) {
+    const bool pre = t < n_pre;
+    const long rs = pre ? p_rs : q_rs;
+    const long at = pre ? (long)t * PKB : (long)lo + (long)(t - n_pre) * PKB;
+    const int rows = min(PKB, (pre ? P : end_row) - (int)at);
+    const long bytes = ((long)(rows - 1) * rs + D) * 2;
+    const desc_t krs = make_desc((pre ? pk : k) + at * rs, bytes);
+    const desc_t vrs = make_desc((pre ? pv : v) + at * rs, bytes);
+    const int rs2 = (int)(rs * 2);
+    const unsigned dst = wave_win + b * 2 * IMG;
+#pragma unroll
+    for (int i = 0; i < NWIN; ++i) {
+      const int off = dma_row[i] * rs2 + dma_col[i];
+      copy16_to_lds(krs, dst + i * 1024, off);
+      copy16_to_lds(vrs, dst + IMG + i * 1024, off);
+    }
+  };
+
+  // LDS read addresses (see the swizzle's row rule in attn_kernels.h)
+  unsigned qk_addr[D / 16];
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk)
+    qk_addr[kk] = swz((unsigned)(lq * (D * 2) + kk * 32 + hi * 16), lq, D64);
+  const int tj = lane & 15;
+  const int tg = (lane >> 4) & 1;
+  unsigned pv_addr[2][D / 32];
+#pragma unroll
+  for (int rd = 0; rd < 2; ++rd) {
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) {
+      const int key0 = 8 * hi + 4 * rd + (tj >> 2);
+      const int dh = db * 32 + 16 * tg + 4 * (tj & 3);
+      pv_addr[rd][db] = swz((unsigned)(key0 * (D * 2) + dh * 2), key0, D64);
+    }
+  }
+  // Both subtiles' scores. All fragments are read before the products: left
+  // to itself the compiler reads each into the same registers and waits.
+  auto scores = [&](int b, f32x16 (&s)[2]) {
+    bf16x8 a[2][D / 16];
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        a[sub][kk] = *(const bf16x8*)(smem + qk_addr[kk] + b * 2 * IMG +
+                                      sub * 32 * (D * 2));
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      s[sub] = alibi;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        s[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[sub][kk], qfrag[kk],
+                                                         s[sub], 0, 0, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, D / 8, 0);  // LDS reads
+    __builtin_amdgcn_sched_group_barrier(0x008, D / 8, 0);  // products
+  };
+  auto add_values = [&](const float* p, int b, int sub) {
+#pragma unroll
+    for (int s16 = 0; s16 < 2; ++s16) {
+      const bf16x8 pf = pack_weights(p + 8 * s16);
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) {
+        union { bf16x4 half[2]; bf16x8 all; } a;
+#pragma unroll
+        for (int rd = 0; rd < 2; ++rd)
+          a.half[rd] = lds_tr16((const __bf16*)(smem + IMG),
+                                pv_addr[rd][db] + b * 2 * IMG +
+                                    sub * 32 * (D * 2) + s16 * 16 * (D * 2));
+        o_acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.all, pf,
+                                                            o_acc[db], 0, 0, 0);
+      }
+    }
+  };
+  // Rescale only when a row's maximum grew by more than 2^8: until then the
+  // weights stay below 2^8 and the sums in range.
+  auto raise = [&](float top) {
+    if (!__all(top - m_run <= 8.f)) {
+      const float m_new = fmaxf(m_run, top);
+      const float a = exp2_fast(m_run - m_new);
+      l_run *= a;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o_acc[db][r] *= a;
+      m_run = m_new;
+    }
+  };
+
+  // A weight of zero does not hide an infinity or NaN among the values it is
+  // multiplied with. Prefix tiles hold nothing that a row may not see; in the
+  // packed rows a value belongs to other sequences or later rows as well. So
+  // values that are not finite are taken out of such a tile (returns whether
+  // there were any) and added by add_bad() where they are seen.
+  int* bad_words = (int*)(smem + lds_images(D, NW));
+  auto take_out_bad = [&](int b) {
+    unsigned* img = (unsigned*)(smem + b * 2 * IMG + IMG);
+    auto bad_half = [](unsigned w, unsigned mask) { return (w & mask) == mask; };
+    bool bad = false;
+    for (int i = threadIdx.x; i < IMG / 4; i += 64 * NW)
+      bad |= bad_half(img[i], 0x7f800000u) || bad_half(img[i], 0x7f80u);
+    const bool wave_bad = __any(bad);
+    if (lane == 0) bad_words[wave] = wave_bad;
+    __syncthreads();
+    bool any = false;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) any |= bad_words[w] != 0;
+    if (!any) return false;
+    for (int i = threadIdx.x; i < IMG / 4; i += 64 * NW) {
+      if (bad_half(img[i], 0x7f800000u)) img[i] &= 0xffffu;
+      if (bad_half(img[i], 0x7f80u)) img[i] &= 0xffff0000u;
+    }
+    __syncthreads();
+    return true;
+  };
+  auto add_bad = [&](int kv0) {
+    const int end = min(kv0 + PKB, end_row);
+#pragma unroll 1
+    for (int key = kv0; key < end; ++key) {
+      const bool seen = key >= first && key <= row;
+      const __bf16* x = v + (long)key * q_rs;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float f = (float)x[db * 32 + (r & 3) + 8 * (r >> 2) + 4 * hi];
+          if (seen && !(fabsf(f) < INFINITY)) o_acc[db][r] += f;
+        }
+    }
+  };
+
+  // From the nearest keys to the farthest: ALiBi makes the weights fall on
+  // the way, so the first tiles set the maximum and the sums are hardly ever
+  // rescaled (forwards, a steep head's maximum rises with every tile).
+  if (t0 < t1) stage(t1 - 1, 0);
+  for (int t = t1 - 1; t >= t0; --t) {
+    const int b = (t1 - 1 - t) & 1;
+    vm_wait0();
+    __syncthreads();  // tile b is there; all reads of the other one are done
+    if (t > t0) stage(t - 1, 1 - b);
+    const bool pre = t < n_pre;
+    const int kv0 = pre ? t * PKB : lo + (t - n_pre) * PKB;
+    const bool masked = !pre || (t + 1) * PKB > P;
+    const bool bad = pre ? false : take_out_bad(b);
+    f32x16 s[2];
+    scores(b, s);
+    if (masked) {
+      // keys from .. from + span of this row, counted from the lane's first
+      const int from = (pre ? 0 : first) - (kv0 + 4 * hi);
+      const unsigned span = pre ? P - 1 : row - first;
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = sub * 32 + (r & 3) + 8 * (r >> 2);
+          if ((unsigned)(key - from) > span) s[sub][r] = -INFINITY;
+        }
+    }
+    const float c = slope2 * (float)(kv0 - (pre ? P + own : row));
+    float x = s[0][0], y = s[1][0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) {
+      x = __builtin_elementwise_maximum(x, s[0][r]);
+      y = __builtin_elementwise_maximum(y, s[1][r]);
+    }
+    const float top = swap_max(__builtin_elementwise_maximum(
+        fmaf(x, scale2, c), fmaf(y, scale2, c + 32.f * slope2)));
+    // Below 2^-150 of the maximum a weight is zero in fp32: a tile of such
+    // weights (far keys of a steep head, other sequences' rows) adds nothing.
+    // A NaN among the scores makes the comparison false.
+    if (!bad && __all(top - m_run < -150.f)) continue;
+    raise(top);
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      const float shift = c + (float)(32 * sub) * slope2 - m_run;
+      float p[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        p[r] = exp2_fast(fmaf(s[sub][r], scale2, shift));
+        l_run += p[r];
+      }
+      add_values(p, b, sub);
+    }
+    if (bad) add_bad(kv0);
+  }
+  l_run += __shfl_xor(l_run, 32, 64);
+  __syncthreads();  // the images are free
+
+  // Through LDS to whole rows. A wave has the 32 x D values of its own rows.
+  if (parts == 1 && !DECODE) {
+    __bf16* o_img = (__bf16*)smem + wave * 32 * D;
+    const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        o_img[lq * D + db * 32 + (r & 3) + 8 * (r >> 2) + 4 * hi] =
+            (__bf16)(o_acc[db][r] * inv);
+    __syncthreads();
+    for (int c = lane; c < 32 * D / 8; c += 64) {
+      const int r = q0_block + wave * QB + c / (D / 8);
+      const int col = (c % (D / 8)) * 8;
+      if (r < T)
+        *(bf16x8*)(out + (long)r * H * D + (long)h * D + col) =
+            *(const bf16x8*)(o_img + c * 8);
+    }
+  } else {
+    float* o_img = (float*)smem + wave * 32 * D;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *(f32x4*)(o_img + lq * D + db * 32 + 2 * r + 4 * hi) =
+            f32x4{o_acc[db][r], o_acc[db][r + 1], o_acc[db][r + 2],
+                  o_acc[db][r + 3]};
+    __syncthreads();
+    // partial rows: [split][item - full][row of the item]
+    const int rest = (T + NW * QB - 1) / (NW * QB) * H - full;
+    const long base =
+        ((long)split * rest + item - full) * (NW * QB) + wave * QB;
+    for (int c = lane; c < 32 * D / 4; c += 64)
+      *(f32x4*)(part_o + base * D + c * 4) = *(const f32x4*)(o_img + c * 4);
+    if (hi == 0) {
+      part_ml[(base + lq) * 2] = m_run;
+      part_ml[(base + lq) * 2 + 1] = l_run;
+    }
+  }
+}
+
+// Joins the splits: a thread has four columns of a row.
+// An item is `rows` rows of one head; the items from `full` on were split.
+template <int D>
+__global__ __launch_bounds__(256) void prefix_join_kernel(
+    const float* __restrict__ part_o, const float* __restrict__ part_ml,
+    __bf16* __restrict__ out, int T, int H, int rows, int full, int rest,
+    int splits) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const long pr = i / (D / 4);  // partial row: [item - full][row]
+  const int col = (int)(i % (D / 4)) * 4;
+  if (pr >= (long)rest * rows) return;
+  const int item = full + (int)(pr / rows);
+  const int h = item % H;
+  const long t = (long)(item / H) * rows + pr % rows;
+  if (t >= T) return;
+  const long stride = (long)rest * rows;
+  float M = -1e30f;
+  for (int s = 0; s < splits; ++s)
+    M = fmaxf(M, part_ml[(s * stride + pr) * 2]);
+  float l = 0.f;
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float w = exp2_fast(part_ml[(s * stride + pr) * 2] - M);
+    l += w * part_ml[(s * stride + pr) * 2 + 1];
+    const f32x4 x = *(const f32x4*)(part_o + (s * stride + pr) * D + col);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] += w * x[j];
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  bf16x4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = (__bf16)(o[j] * inv);
+  *(bf16x4*)(out + (t * H + h) * D + col) = r;
+}
+
+// Decode: one workgroup per (sequence, head) writes the new key and value to
+// the cache, attends the sequence's own keys and joins what the prefix gave.
+// D / 8 lanes hold a key's 8 columns each, all groups of the block stride
+// over the keys with a running maximum and sum of their own.
+constexpr int OWN_BLOCK = 256;
+template <int D>
+__global__ __launch_bounds__(OWN_BLOCK) void decode_own_kernel(
+    const __bf16* __restrict__ qkv, long q_rs, __bf16* __restrict__ cache,
+    long c_bs, long c_ss, long c_ks, long c_hs,
+    const float* __restrict__ slopes, const int* __restrict__ held,
+    const float* __restrict__ part_o, const float* __restrict__ part_ml,
+    __bf16* __restrict__ out, int H, int slots, int rows, int items,
+    int splits) {
+  constexpr int L = D / 8;               // lanes a key
+  constexpr int G = OWN_BLOCK / L;       // keys at a time
+  __shared__ float s_o[OWN_BLOCK / 64][D];
+  __shared__ float s_m[OWN_BLOCK / 64], s_l[OWN_BLOCK / 64];
+  const int h = blockIdx.x;
+  const int b = blockIdx.y;
+  const int tid = threadIdx.x;
+  const int g = tid / L;
+  const int c = (tid % L) * 8;
+  const __bf16* q = qkv + b * q_rs + (long)h * D;
+  const int n = held[b];
+  __bf16* o_row = out + ((long)b * H + h) * D;
+  if (n < 0 || n >= slots) {  // no room for the new key: say so
+    if (tid < D) o_row[tid] = (__bf16)__builtin_nanf("");
+    return;
+  }
+  __bf16* ck = cache + b * c_bs + (long)h * c_hs;
+  __bf16* cv = ck + c_ks;
+  const bf16x8 new_k = *(const bf16x8*)(q + (long)H * D + c);
+  const bf16x8 new_v = *(const bf16x8*)(q + 2L * H * D + c);
+  if (g == 0) {
+    *(bf16x8*)(ck + (long)n * c_ss + c) = new_k;
+    *(bf16x8*)(cv + (long)n * c_ss + c) = new_v;
+  }
+  float qf[8];
+  const bf16x8 qv = *(const bf16x8*)(q + c);
+  const float scale2 = rsqrtf((float)D) * LOG2E;
+  const float slope2 = slopes[h] * LOG2E;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) qf[j] = (float)qv[j] * scale2;
+  float m = -1e30f, l = 0.f, o[8] = {};
+  for (int i = g; i <= n; i += G) {
+    bf16x8 kv = new_k, vv = new_v;  // the new ones from registers
+    if (i < n) {
+      kv = *(const bf16x8*)(ck + (long)i * c_ss + c);
+      vv = *(const bf16x8*)(cv + (long)i * c_ss + c);
+    }
+    float w = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w = fmaf(qf[j], (float)kv[j], w);
+#pragma unroll
+    for (int off = L / 2; off > 0; off >>= 1) w += __shfl_xor(w, off, WAVE);
+    w -= slope2 * (float)(n - i);
+    const float m_new = fmaxf(m, w);
+    const float a = exp2_fast(m - m_new);
+    const float p = exp2_fast(w - m_new);
+    m = m_new;
+    l = l * a + p;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = fmaf(p, (float)vv[j], o[j] * a);
+  }
+  // the wave's groups, then the block's waves
+#pragma unroll
+  for (int off = L; off < WAVE; off <<= 1) {
+    const float m2 = __shfl_xor(m, off, WAVE);
+    const float l2 = __shfl_xor(l, off, WAVE);
+    const float M = fmaxf(m, m2);
+    const float a = exp2_fast(m - M), a2 = exp2_fast(m2 - M);
+    m = M;
+    l = l * a + l2 * a2;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      o[j] = o[j] * a + __shfl_xor(o[j], off, WAVE) * a2;
+  }
+  const int wave = tid >> 6;
+  if ((tid & 63) < L) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s_o[wave][c + j] = o[j];
+    if ((tid & 63) == 0) {
+      s_m[wave] = m;
+      s_l[wave] = l;
+    }
+  }
+  __syncthreads();
+  if (tid >= D) return;
+  // the sequence's row of the prefix's partial ones
+  const long stride = (long)items * rows;
+  const long rh = ((long)(b / rows) * H + h) * rows + b % rows;
+  float M = -1e30f;
+  for (int s = 0; s < splits; ++s)
+    M = fmaxf(M, part_ml[(s * stride + rh) * 2]);
+#pragma unroll
+  for (int w = 0; w < OWN_BLOCK / 64; ++w) M = fmaxf(M, s_m[w]);
+  float sum = 0.f, acc = 0.f;
+#pragma unroll
+  for (int w = 0; w < OWN_BLOCK / 64; ++w) {
+    const float a = exp2_fast(s_m[w] - M);
+    sum += a * s_l[w];
+    acc += a * s_o[w][tid];
+  }
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float a = exp2_fast(part_ml[(s * stride + rh) * 2] - M);
+    sum += a * part_ml[(s * stride + rh) * 2 + 1];
+    acc += a * part_o[(s * stride + rh) * D + tid];
+  }
+  o_row[tid] = (__bf16)(acc / sum);
+}
+
+}  // namespace photon_hip
