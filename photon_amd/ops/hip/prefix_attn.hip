@@ -22,14 +22,16 @@ struct Cut {
 // Whole rounds of items fill the chip by themselves; what is left over is
 // split until it does, but not below two key tiles each. `always`: every item
 // leaves partial rows.
-Cut cut(long T, int H, int key_tiles, bool always) {
+Cut cut(long T, int H, int D, int key_tiles, bool always) {
   Cut c;
   c.waves = T <= 32 ? 1 : T <= 64 ? 2 : 4;
   c.rows = c.waves * QB;
   const long items = (T + c.rows - 1) / c.rows * H;
   TORCH_CHECK(items < (1L << 22), "prefix attention: too many rows");
   c.items = (int)items;
-  const int at_once = 512;
+  // a CU holds two workgroups of four waves (three with short heads), or one
+  // with four buffers
+  const int at_once = c.waves < 4 ? 256 : D == 64 ? 768 : 512;
   c.full = always ? 0 : c.items / at_once * at_once;
   c.rest = c.items - c.full;
   c.splits = 1;
@@ -54,18 +56,21 @@ void launch(const torch::Tensor& qkv, const torch::Tensor& prefix, int H,
   cur_stream(), (const __bf16*)qkv.data_ptr(), qkv.stride(0), pk, pv,        \
       prefix.stride(0), slopes.data_ptr<float>(), info.data_ptr<int>(), out, \
       part_o, part_ml, T, P, H, c.full, c.splits
-#define LAUNCH(DD, NW)                                                       \
-  hipLaunchKernelGGL((prefix_attn_kernel<DD, NW, DECODE>), dim3(c.groups()), \
-                     dim3(64 * NW), lds_bytes(DD, NW), ARGS)
+#define LAUNCH(DD, NW, BUFS)                                                 \
+  hipLaunchKernelGGL((prefix_attn_kernel<DD, NW, BUFS, DECODE>),             \
+                     dim3(c.groups()), dim3(64 * NW),                        \
+                     lds_bytes(DD, NW, BUFS), ARGS)
+#define LAUNCH_D(DD)                                                         \
+  if (c.waves == 1) { LAUNCH(DD, 1, 4); }                                    \
+  else if (c.waves == 2) { LAUNCH(DD, 2, 4); }                               \
+  else if (c.groups() <= 256) { LAUNCH(DD, 4, 4); }                          \
+  else { LAUNCH(DD, 4, 2); }
   if (D == 64) {
-    if (c.waves == 1) { LAUNCH(64, 1); }
-    else if (c.waves == 2) { LAUNCH(64, 2); }
-    else { LAUNCH(64, 4); }
+    LAUNCH_D(64)
   } else {
-    if (c.waves == 1) { LAUNCH(128, 1); }
-    else if (c.waves == 2) { LAUNCH(128, 2); }
-    else { LAUNCH(128, 4); }
+    LAUNCH_D(128)
   }
+#undef LAUNCH_D
 #undef LAUNCH
 #undef ARGS
 }
@@ -126,7 +131,7 @@ torch::Tensor prefix_attention(torch::Tensor qkv, torch::Tensor prefix, long H,
   const Args a = check(qkv, prefix, H, slopes, starts);
   auto out = torch::empty({(long)a.T, (long)a.H * a.D}, qkv.options());
   if (a.T == 0) return out;
-  const Cut c = cut(a.T, a.H, (a.P + PKB - 1) / PKB + 1, false);
+  const Cut c = cut(a.T, a.H, a.D, (a.P + PKB - 1) / PKB + 1, false);
   torch::Tensor po, pm;
   if (c.rest) {
     auto f = qkv.options().dtype(at::kFloat);
@@ -174,7 +179,7 @@ torch::Tensor prefix_attention_decode(torch::Tensor qkv, torch::Tensor prefix,
   Cut c{};
   torch::Tensor po, pm;
   if (a.P > 0) {
-    c = cut(B, a.H, (a.P + PKB - 1) / PKB, true);
+    c = cut(B, a.H, a.D, (a.P + PKB - 1) / PKB, true);
     auto f = qkv.options().dtype(at::kFloat);
     po = torch::empty({c.partial_rows() * a.D}, f);
     pm = torch::empty({c.partial_rows() * 2}, f);

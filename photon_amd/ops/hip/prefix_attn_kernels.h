@@ -55,6 +55,12 @@ DEV_INLINE void copy16_to_lds(desc_t desc, unsigned lds, int offset) {
       : "memory", "m0");
 }
 
+// Until at most N of this wave's copies are on their way (in order).
+template <int N>
+DEV_INLINE void vm_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 // The larger of a row's two halves (lanes l and l + 32); NaN if one is.
 DEV_INLINE float swap_max(float x) {
   union { float f; unsigned u; } a, b;
@@ -85,13 +91,15 @@ DEV_INLINE bf16x8 pack_weights(const float* p) {
   return out.v;
 }
 
-// LDS: two buffers of a key and a value image (or, at the end, the fp32 rows
-// of all waves), and a word for each wave.
-constexpr int lds_images(int D, int nw) {
-  const int images = 4 * PKB * D * 2, rows = nw * 32 * D * 4;
+// LDS: `bufs` buffers of a key and a value image (or, at the end, the fp32
+// rows of all waves), and a word for each wave.
+constexpr int lds_images(int D, int nw, int bufs) {
+  const int images = bufs * 2 * PKB * D * 2, rows = nw * 32 * D * 4;
   return images > rows ? images : rows;
 }
-constexpr int lds_bytes(int D, int nw) { return lds_images(D, nw) + 64; }
+constexpr int lds_bytes(int D, int nw, int bufs) {
+  return lds_images(D, nw, bufs) + 64;
+}
 
 // Swapped product (keys x queries): lane holds query lane & 31, its 16
 // registers the keys (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5) of 32.
@@ -99,8 +107,12 @@ constexpr int lds_bytes(int D, int nw) { return lds_images(D, nw) + 64; }
 // `info` is each row's first own row (packed form) or, in the decode form, how
 // many own keys the row's sequence holds; there the kernel covers the prefix
 // only.
-template <int D, int NW, bool DECODE>
-__global__ __launch_bounds__(64 * NW, 2) void prefix_attn_kernel(
+//
+// BUFS key tiles are in LDS or on their way. Two, and two workgroups a CU,
+// where there are many; four where a CU has one at most and nothing else hides
+// the way from memory.
+template <int D, int NW, int BUFS, bool DECODE>
+__global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void prefix_attn_kernel(
     const __bf16* __restrict__ qkv, long q_rs, const __bf16* __restrict__ pk,
     const __bf16* __restrict__ pv, long p_rs,
     const float* __restrict__ slopes, const int* __restrict__ info,
@@ -159,8 +171,9 @@ __global__ __launch_bounds__(64 * NW, 2) void prefix_attn_kernel(
     n_own = (end_row - lo + PKB - 1) / PKB;
   }
   const int n_all = n_pre + n_own;
-  const int t0 = (int)((long)n_all * split / parts);
-  const int t1 = (int)((long)n_all * (split + 1) / parts);
+  const int each = n_all / parts, more = n_all - each * parts;
+  const int t0 = split * each + min(split, more);
+  const int t1 = t0 + each + (split < more ? 1 : 0);
 
   float m_run = -1e30f;  // finite: exp2(-huge) == 0 and no NaN from inf - inf
   float l_run = 0.f;      // this half's share of the sum
@@ -286,13 +299,22 @@ __global__ __launch_bounds__(64 * NW, 2) void prefix_attn_kernel(
   // packed rows a value belongs to other sequences or later rows as well. So
   // values that are not finite are taken out of such a tile (returns whether
   // there were any) and added by add_bad() where they are seen.
-  int* bad_words = (int*)(smem + lds_images(D, NW));
+  int* bad_words = (int*)(smem + lds_images(D, NW, BUFS));
   auto take_out_bad = [&](int b) {
-    unsigned* img = (unsigned*)(smem + b * 2 * IMG + IMG);
+    uint4* img = (uint4*)(smem + b * 2 * IMG + IMG);
+    constexpr int EACH = IMG / 16 / (64 * NW);
     auto bad_half = [](unsigned w, unsigned mask) { return (w & mask) == mask; };
+    auto bad_word = [&](unsigned w) {
+      return bad_half(w, 0x7f800000u) | bad_half(w, 0x7f80u);
+    };
+    uint4 w[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) w[i] = img[threadIdx.x + i * 64 * NW];
     bool bad = false;
-    for (int i = threadIdx.x; i < IMG / 4; i += 64 * NW)
-      bad |= bad_half(img[i], 0x7f800000u) || bad_half(img[i], 0x7f80u);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      bad |= bad_word(w[i].x) | bad_word(w[i].y) | bad_word(w[i].z) |
+             bad_word(w[i].w);
     const bool wave_bad = __any(bad);
     if (lane == 0) bad_words[wave] = wave_bad;
     __syncthreads();
@@ -300,9 +322,11 @@ __global__ __launch_bounds__(64 * NW, 2) void prefix_attn_kernel(
 #pragma unroll
     for (int w = 0; w < NW; ++w) any |= bad_words[w] != 0;
     if (!any) return false;
+    unsigned* words = (unsigned*)img;
+#pragma unroll 1
     for (int i = threadIdx.x; i < IMG / 4; i += 64 * NW) {
-      if (bad_half(img[i], 0x7f800000u)) img[i] &= 0xffffu;
-      if (bad_half(img[i], 0x7f80u)) img[i] &= 0xffff0000u;
+      if (bad_half(words[i], 0x7f800000u)) words[i] &= 0xffffu;
+      if (bad_half(words[i], 0x7f80u)) words[i] &= 0xffff0000u;
     }
     __syncthreads();
     return true;
@@ -326,12 +350,20 @@ __global__ __launch_bounds__(64 * NW, 2) void prefix_attn_kernel(
   // From the nearest keys to the farthest: ALiBi makes the weights fall on
   // the way, so the first tiles set the maximum and the sums are hardly ever
   // rescaled (forwards, a steep head's maximum rises with every tile).
-  if (t0 < t1) stage(t1 - 1, 0);
+#pragma unroll
+  for (int i = 0; i < BUFS - 1; ++i)
+    if (t1 - 1 - i >= t0) stage(t1 - 1 - i, i);
+  int b = BUFS - 1;
   for (int t = t1 - 1; t >= t0; --t) {
-    const int b = (t1 - 1 - t) & 1;
-    vm_wait0();
-    __syncthreads();  // tile b is there; all reads of the other one are done
-    if (t > t0) stage(t - 1, 1 - b);
+    const int old = b;  // the buffer of tile t + 1
+    b = b == BUFS - 1 ? 0 : b + 1;
+    // the copies of the BUFS - 2 tiles behind t may still be on their way
+    if (t - t0 >= BUFS - 2)
+      vm_wait<(BUFS - 2) * 2 * NWIN < 63 ? (BUFS - 2) * 2 * NWIN : 63>();
+    else
+      vm_wait0();
+    __syncthreads();  // tile t is there; all reads of tile t + 1 are done
+    if (t - (BUFS - 1) >= t0) stage(t - (BUFS - 1), old);
     const bool pre = t < n_pre;
     const int kv0 = pre ? t * PKB : lo + (t - n_pre) * PKB;
     const bool masked = !pre || (t + 1) * PKB > P;
@@ -438,11 +470,12 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(
   if (t >= T) return;
   const long stride = (long)rest * rows;
   float M = -1e30f;
+#pragma unroll 8
   for (int s = 0; s < splits; ++s)
     M = fmaxf(M, part_ml[(s * stride + pr) * 2]);
   float l = 0.f;
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+#pragma unroll 8
   for (int s = 0; s < splits; ++s) {
     const float w = exp2_fast(part_ml[(s * stride + pr) * 2] - M);
     l += w * part_ml[(s * stride + pr) * 2 + 1];
@@ -501,25 +534,47 @@ __global__ __launch_bounds__(OWN_BLOCK) void decode_own_kernel(
 #pragma unroll
   for (int j = 0; j < 8; ++j) qf[j] = (float)qv[j] * scale2;
   float m = -1e30f, l = 0.f, o[8] = {};
-  for (int i = g; i <= n; i += G) {
-    bf16x8 kv = new_k, vv = new_v;  // the new ones from registers
-    if (i < n) {
-      kv = *(const bf16x8*)(ck + (long)i * c_ss + c);
-      vv = *(const bf16x8*)(cv + (long)i * c_ss + c);
+  // U keys at a time, all their loads in flight together and one rescaling
+  constexpr int U = 4;
+  for (int i0 = g; i0 <= n; i0 += U * G) {
+    bf16x8 kv[U], vv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * G;
+      kv[u] = new_k;  // the new ones from registers
+      vv[u] = new_v;
+      if (i < n) {
+        kv[u] = *(const bf16x8*)(ck + (long)i * c_ss + c);
+        vv[u] = *(const bf16x8*)(cv + (long)i * c_ss + c);
+      }
     }
-    float w = 0.f;
+    float w[U];
+    float m_new = m;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w = fmaf(qf[j], (float)kv[j], w);
+    for (int u = 0; u < U; ++u) {
+      float x = 0.f;
 #pragma unroll
-    for (int off = L / 2; off > 0; off >>= 1) w += __shfl_xor(w, off, WAVE);
-    w -= slope2 * (float)(n - i);
-    const float m_new = fmaxf(m, w);
+      for (int j = 0; j < 8; ++j) x = fmaf(qf[j], (float)kv[u][j], x);
+#pragma unroll
+      for (int off = L / 2; off > 0; off >>= 1) x += __shfl_xor(x, off, WAVE);
+      const int i = i0 + u * G;
+      w[u] = i <= n ? x - slope2 * (float)(n - i) : -INFINITY;
+      m_new = fmaxf(m_new, w[u]);
+    }
     const float a = exp2_fast(m - m_new);
-    const float p = exp2_fast(w - m_new);
     m = m_new;
-    l = l * a + p;
+    l *= a;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = fmaf(p, (float)vv[j], o[j] * a);
+    for (int j = 0; j < 8; ++j) o[j] *= a;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u * G <= n) {  // a value behind the new one is not touched
+        const float p = exp2_fast(w[u] - m);
+        l += p;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = fmaf(p, (float)vv[u][j], o[j]);
+      }
+    }
   }
   // the wave's groups, then the block's waves
 #pragma unroll
@@ -549,6 +604,7 @@ __global__ __launch_bounds__(OWN_BLOCK) void decode_own_kernel(
   const long stride = (long)items * rows;
   const long rh = ((long)(b / rows) * H + h) * rows + b % rows;
   float M = -1e30f;
+#pragma unroll 8
   for (int s = 0; s < splits; ++s)
     M = fmaxf(M, part_ml[(s * stride + rh) * 2]);
 #pragma unroll
@@ -560,7 +616,7 @@ __global__ __launch_bounds__(OWN_BLOCK) void decode_own_kernel(
     sum += a * s_l[w];
     acc += a * s_o[w][tid];
   }
-#pragma unroll 4
+#pragma unroll 8
   for (int s = 0; s < splits; ++s) {
     const float a = exp2_fast(part_ml[(s * stride + rh) * 2] - M);
     sum += a * part_ml[(s * stride + rh) * 2 + 1];
