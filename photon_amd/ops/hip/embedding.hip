@@ -106,16 +106,35 @@ __global__ __launch_bounds__(EMB_BLOCK) void embed_fwd_kernel(
 // ---------------------------------------------------------------------------
 // Backward, step 1: stable radix sort of (token, position), 8 bits a pass.
 //
-// A block owns `tile` consecutive items; counts[block][digit] of a pass are
-// made by the pass before (by a kernel of their own for the first one), and
-// every scatter block derives its places from all blocks' counts, which
-// stands for a scan kernel in between. At most SORT_BLOCKS blocks, so that
-// these counts stay at 128 KiB.
+// A block owns `rounds` * SORT_TILE consecutive items; counts[block][digit] of
+// a pass are made by the pass before (by a kernel of their own for the first
+// one), and every scatter block derives its places from all blocks' counts,
+// which stands for a scan kernel in between. At most SORT_BLOCKS blocks, so
+// that these counts stay at 128 KiB.
+//
+// The sort is bound by latencies and leaves the memory idle; the blocks behind
+// the sorting ones use that time to clear the gradient, a share in each kernel
+// (a row that has tokens is written again by step 2).
 // ---------------------------------------------------------------------------
 constexpr int SORT_BLOCKS = 128;
-constexpr int SORT_TILE = 1024;
+constexpr int ITEMS = 4;  // a lane and round
+constexpr int SORT_TILE = EMB_BLOCK * ITEMS;
 constexpr int DIGITS = 256;
 constexpr int SORT_WAVES = EMB_BLOCK / WAVE;
+
+struct Fill {
+  uint4* p;   // aligned to 16 bytes
+  long n;     // 16-byte words
+  int first;  // first block that clears
+};
+
+DEV_INLINE void clear(const Fill& f) {
+  const long step = (long)(gridDim.x - f.first) * EMB_BLOCK;
+#pragma unroll 4
+  for (long i = (long)(blockIdx.x - f.first) * EMB_BLOCK + threadIdx.x; i < f.n;
+       i += step)
+    f.p[i] = uint4{0, 0, 0, 0};
+}
 
 template <typename I>
 DEV_INLINE unsigned token_key(const I* ids, long i, long V) {
@@ -125,20 +144,23 @@ DEV_INLINE unsigned token_key(const I* ids, long i, long V) {
 
 template <typename I>
 __global__ __launch_bounds__(EMB_BLOCK) void sort_count_kernel(
-    const I* __restrict__ ids, int N, long V, int tile,
-    unsigned* __restrict__ counts, int more_passes) {
+    const I* __restrict__ ids, int N, long V, int rounds,
+    unsigned* __restrict__ counts, int more_passes, const Fill fill) {
+  if ((int)blockIdx.x >= fill.first) return clear(fill);
   __shared__ unsigned hist[DIGITS];
   hist[threadIdx.x] = 0;
   __syncthreads();
-  const long b0 = (long)blockIdx.x * tile;
+  const long tile = (long)rounds * SORT_TILE;
+  const long b0 = blockIdx.x * tile;
   const long b1 = min(b0 + tile, (long)N);
+#pragma unroll 4
   for (long i = b0 + threadIdx.x; i < b1; i += EMB_BLOCK)
     atomicAdd(&hist[token_key(ids, i, V) & 255u], 1u);
   __syncthreads();
   const int at = blockIdx.x * DIGITS + threadIdx.x;
   counts[at] = hist[threadIdx.x];
   // the following passes' counts start at zero
-  const int stride = gridDim.x * DIGITS;
+  const int stride = fill.first * DIGITS;
   for (int p = 1; p <= more_passes; ++p) counts[p * stride + at] = 0;
 }
 
@@ -146,42 +168,64 @@ template <typename I, bool FIRST>
 __global__ __launch_bounds__(EMB_BLOCK) void sort_scatter_kernel(
     const I* __restrict__ ids, const unsigned* __restrict__ keys_in,
     const unsigned* __restrict__ pos_in, unsigned* __restrict__ keys_out,
-    unsigned* __restrict__ pos_out, int N, long V, int tile, int shift,
-    const unsigned* __restrict__ counts, unsigned* __restrict__ next_counts) {
+    unsigned* __restrict__ pos_out, int N, long V, int rounds, int shift,
+    const unsigned* __restrict__ counts, unsigned* __restrict__ next_counts,
+    const Fill fill) {
+  if ((int)blockIdx.x >= fill.first) return clear(fill);
   __shared__ unsigned offs[SORT_WAVES][DIGITS];
-  __shared__ unsigned totals[DIGITS];
+  __shared__ unsigned wave_totals[SORT_WAVES];
   const int tid = threadIdx.x;
   const int lane = tid & (WAVE - 1);
   const int wid = tid / WAVE;
-  const int nblk = gridDim.x;
+  const int nblk = fill.first;
+  const long tile = (long)rounds * SORT_TILE;
+
+  // a wave owns a quarter of the tile, in order; a round's items are loaded
+  // together
+  const long per_wave = tile / SORT_WAVES;
+  const long w0 = blockIdx.x * tile + wid * per_wave;
+  const long w1 = min(w0 + per_wave, (long)N);
+  unsigned key[ITEMS], pos[ITEMS];
+  auto load = [&](int round) {
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      const long i = w0 + ((long)round * ITEMS + j) * WAVE + lane;
+      key[j] = pos[j] = 0;
+      if (i < w1) {
+        key[j] = FIRST ? token_key(ids, i, V) : keys_in[i];
+        pos[j] = FIRST ? (unsigned)i : pos_in[i];
+      }
+    }
+  };
+  load(0);
 
   // this thread's digit: items in earlier blocks, and in all blocks
   unsigned before = 0, total = 0;
-#pragma unroll 16
+#pragma unroll 32
   for (int b = 0; b < nblk; ++b) {
     const unsigned c = counts[b * DIGITS + tid];
     total += c;
     before += b < (int)blockIdx.x ? c : 0u;
   }
-  totals[tid] = total;
 #pragma unroll
   for (int w = 0; w < SORT_WAVES; ++w) offs[w][tid] = 0;
-  __syncthreads();
-  for (int d = 1; d < DIGITS; d <<= 1) {  // inclusive scan over the digits
-    const unsigned x = tid >= d ? totals[tid - d] : 0u;
-    __syncthreads();
-    totals[tid] += x;
-    __syncthreads();
+  unsigned scan = total;  // inclusive, over the wave's digits
+#pragma unroll
+  for (int d = 1; d < WAVE; d <<= 1) {
+    const unsigned x = __shfl_up(scan, d, WAVE);
+    if (lane >= d) scan += x;
   }
-  const unsigned base = totals[tid] - total + before;
+  if (lane == WAVE - 1) wave_totals[wid] = scan;
+  __syncthreads();
+  unsigned base = scan - total + before;
+  for (int w = 0; w < wid; ++w) base += wave_totals[w];
 
-  // a wave owns a quarter of the tile, in order
-  const int per_wave = tile / SORT_WAVES;
-  const long w0 = (long)blockIdx.x * tile + (long)wid * per_wave;
-  const long w1 = min(w0 + per_wave, (long)N);
-  for (long i = w0 + lane; i < w1; i += WAVE) {
-    const unsigned k = FIRST ? token_key(ids, i, V) : keys_in[i];
-    atomicAdd(&offs[wid][(k >> shift) & 255u], 1u);
+  for (int r = 0; r < rounds; ++r) {
+    if (r > 0) load(r);
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+      if (w0 + ((long)r * ITEMS + j) * WAVE + lane < w1)
+        atomicAdd(&offs[wid][(key[j] >> shift) & 255u], 1u);
   }
   __syncthreads();
   unsigned run = base;
@@ -193,35 +237,34 @@ __global__ __launch_bounds__(EMB_BLOCK) void sort_scatter_kernel(
   }
   __syncthreads();
   volatile unsigned* mine = offs[wid];
-  for (long i0 = w0; i0 < w1; i0 += WAVE) {
-    const long i = i0 + lane;
-    const bool live = i < w1;
-    unsigned k = 0, pos = 0;
-    if (live) {
-      k = FIRST ? token_key(ids, i, V) : keys_in[i];
-      pos = FIRST ? (unsigned)i : pos_in[i];
-    }
-    const unsigned digit = (k >> shift) & 255u;
-    unsigned long long same = __ballot(live);
+  for (int r = 0; r < rounds; ++r) {
+    if (rounds > 1) load(r);
 #pragma unroll
-    for (int bit = 0; bit < 8; ++bit) {
-      const unsigned long long one = __ballot((digit >> bit) & 1u);
-      same &= ((digit >> bit) & 1u) ? one : ~one;
-    }
-    if (live) {
-      const int rank = __popcll(same & ((1ull << lane) - 1ull));
-      const unsigned at = mine[digit];
+    for (int j = 0; j < ITEMS; ++j) {
+      const bool live = w0 + ((long)r * ITEMS + j) * WAVE + lane < w1;
+      const unsigned k = key[j];
+      const unsigned digit = (k >> shift) & 255u;
+      unsigned long long same = __ballot(live);
+#pragma unroll
+      for (int bit = 0; bit < 8; ++bit) {
+        const unsigned long long one = __ballot((digit >> bit) & 1u);
+        same &= ((digit >> bit) & 1u) ? one : ~one;
+      }
+      if (live) {
+        const int rank = __popcll(same & ((1ull << lane) - 1ull));
+        const unsigned at = mine[digit];
+        __builtin_amdgcn_wave_barrier();
+        if (rank == 0) mine[digit] = at + (unsigned)__popcll(same);
+        const unsigned dst = at + rank;
+        keys_out[dst] = k;
+        pos_out[dst] = pos[j];
+        if (next_counts)
+          atomicAdd(&next_counts[(dst / (unsigned)tile) * DIGITS +
+                                 ((k >> (shift + 8)) & 255u)],
+                    1u);
+      }
       __builtin_amdgcn_wave_barrier();
-      if (rank == 0) mine[digit] = at + (unsigned)__popcll(same);
-      const unsigned dst = at + rank;
-      keys_out[dst] = k;
-      pos_out[dst] = pos;
-      if (next_counts)
-        atomicAdd(&next_counts[(dst / (unsigned)tile) * DIGITS +
-                               ((k >> (shift + 8)) & 255u)],
-                  1u);
     }
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -229,44 +272,19 @@ __global__ __launch_bounds__(EMB_BLOCK) void sort_scatter_kernel(
 // Backward, step 2: sums over CHUNK sorted positions, COLS columns a wave.
 // A segment (one token's positions) inside its chunk is final; one that came
 // from the chunk before goes to head[chunk], one that goes on to the next
-// (and began here) to tail[chunk]. The blocks behind the sums' write the zero
-// rows: each lane looks its token up in the sorted keys.
+// (and began here) to tail[chunk].
 // ---------------------------------------------------------------------------
 constexpr int CHUNK = 32;
-constexpr int FILL_ROWS = 16;  // table rows a filling wave looks after
 
 template <typename TG, typename TW, int VEC>
 __global__ __launch_bounds__(EMB_BLOCK) void embed_sum_kernel(
     const TG* __restrict__ dy, const unsigned* __restrict__ keys,
     const unsigned* __restrict__ pos, TW* __restrict__ dw,
     float* __restrict__ head, float* __restrict__ tail, int N, int D, long V,
-    float scale, int sum_blocks) {
+    float scale) {
   constexpr int COLS = WAVE * VEC;
   const int lane = threadIdx.x & (WAVE - 1);
   const int wid = threadIdx.x / WAVE;
-  if ((int)blockIdx.x >= sum_blocks) {
-    const long r0 =
-        ((long)(blockIdx.x - sum_blocks) * SORT_WAVES + wid) * FILL_ROWS;
-    const long r = r0 + lane;
-    bool absent = false;
-    if (lane < FILL_ROWS && r < V) {
-      int lo = 0, hi = N;  // first sorted position with key >= r
-      while (lo < hi) {
-        const int mid = lo + (hi - lo) / 2;
-        if (keys[mid] < (unsigned)r) lo = mid + 1; else hi = mid;
-      }
-      absent = lo == N || keys[lo] != (unsigned)r;
-    }
-    unsigned long long todo = __ballot(absent);
-    const float zero[VEC] = {};
-    while (todo) {
-      const int i = __ffsll(todo) - 1;
-      todo &= todo - 1;
-      for (int c = lane * VEC; c < D; c += COLS)
-        store_vec<VEC, TW>(dw + (r0 + i) * D + c, zero);
-    }
-    return;
-  }
   const int tiles = (D + COLS - 1) / COLS;
   const long item = (long)blockIdx.x * SORT_WAVES + wid;
   const long chunk = item / tiles;
@@ -324,7 +342,8 @@ __global__ __launch_bounds__(EMB_BLOCK) void embed_sum_kernel(
 
 // Step 3: a token that leaves the chunk it began in is that chunk's tail and
 // the heads of the chunks up to the one that holds its last position. The
-// block's waves take every fourth of them and are added in order.
+// block's waves take every fourth of them and are added in order. One block
+// for each chunk and column tile; most find nothing to join.
 template <typename TW, int VEC>
 __global__ __launch_bounds__(EMB_BLOCK) void embed_join_kernel(
     const unsigned* __restrict__ keys, const float* __restrict__ head,
@@ -339,41 +358,45 @@ __global__ __launch_bounds__(EMB_BLOCK) void embed_join_kernel(
   const long end = first + CHUNK;  // first position of the next chunk
   if (end >= N) return;
   const unsigned k = keys[end - 1];
-  if (keys[end] != k || k >= (unsigned)V) return;
-  if (first > 0 && keys[first] == k && keys[first - 1] == k) return;
-  long lo = end, hi = N;  // first position after the token's
-  while (lo < hi) {
-    const long mid = lo + (hi - lo) / 2;
-    if (keys[mid] <= k) lo = mid + 1; else hi = mid;
+  const unsigned k_next = keys[end];
+  const unsigned k_first = keys[first];
+  const unsigned k_before = keys[max(first - 1, 0L)];
+  const unsigned k_far = keys[min(end + CHUNK, (long)N) - 1];
+  if (k_next != k || k >= (unsigned)V) return;
+  if (first > 0 && k_first == k && k_before == k) return;
+  long last = chunk + 1;  // heads chunk + 1 .. last
+  if (k_far == k) {
+    long lo = end, hi = N;  // first position after the token's
+    while (lo < hi) {
+      const long mid = lo + (hi - lo) / 2;
+      if (keys[mid] <= k) lo = mid + 1; else hi = mid;
+    }
+    last = (lo - 1) / CHUNK;
   }
-  const long last = (lo - 1) / CHUNK;  // heads chunk + 1 .. last
-  for (int c0 = 0; c0 < D; c0 += COLS) {
-    const int c = c0 + lane * VEC;
-    float acc[VEC] = {};
-    if (c < D) {
-      if (wid == 0) load_vec<VEC, float>(tail + chunk * D + c, acc);
-#pragma unroll 4
-      for (long h = chunk + 1 + wid; h <= last; h += SORT_WAVES) {
-        float f[VEC];
-        load_vec<VEC, float>(head + h * D + c, f);
+  const int c = blockIdx.y * COLS + lane * VEC;
+  float acc[VEC] = {};
+  if (c < D) {
+    if (wid == 0) load_vec<VEC, float>(tail + chunk * D + c, acc);
+#pragma unroll 8
+    for (long h = chunk + 1 + wid; h <= last; h += SORT_WAVES) {
+      float f[VEC];
+      load_vec<VEC, float>(head + h * D + c, f);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] += f[j];
-      }
+      for (int j = 0; j < VEC; ++j) acc[j] += f[j];
     }
-    __syncthreads();
+  }
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) sums[wid][lane * VEC + j] = acc[j];
-    __syncthreads();
-    if (wid == 0 && c < D) {
+  for (int j = 0; j < VEC; ++j) sums[wid][lane * VEC + j] = acc[j];
+  __syncthreads();
+  if (wid == 0 && c < D) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float s = sums[0][lane * VEC + j];
+    for (int j = 0; j < VEC; ++j) {
+      float s = sums[0][lane * VEC + j];
 #pragma unroll
-        for (int w = 1; w < SORT_WAVES; ++w) s += sums[w][lane * VEC + j];
-        acc[j] = s * scale;
-      }
-      store_vec<VEC, TW>(dw + (long)k * D + c, acc);
+      for (int w = 1; w < SORT_WAVES; ++w) s += sums[w][lane * VEC + j];
+      acc[j] = s * scale;
     }
+    store_vec<VEC, TW>(dw + (long)k * D + c, acc);
   }
 }
 
@@ -451,10 +474,9 @@ torch::Tensor embedding_bwd(const torch::Tensor& dy_in,
   if (N == 0) return dw.zero_();
   int passes = 1;
   while (passes < 4 && (V >> (8 * passes)) != 0) ++passes;
-  // tiles of at least SORT_TILE, at most SORT_BLOCKS of them
-  const long tiles = std::min<long>((N + SORT_TILE - 1) / SORT_TILE, SORT_BLOCKS);
-  const int tile =
-      (int)(((N + tiles - 1) / tiles + EMB_BLOCK - 1) / EMB_BLOCK * EMB_BLOCK);
+  const int rounds =
+      (int)((N + (long)SORT_TILE * SORT_BLOCKS - 1) / ((long)SORT_TILE * SORT_BLOCKS));
+  const long tile = (long)rounds * SORT_TILE;
   const int nblk = (int)((N + tile - 1) / tile);
   const long chunks = (N + CHUNK - 1) / CHUNK;
 
@@ -466,23 +488,34 @@ torch::Tensor embedding_bwd(const torch::Tensor& dy_in,
   unsigned* cp = (unsigned*)counts.data_ptr();
   const auto stream = cur_stream();
   int at_pair = 0;
+  // The gradient's 16-byte words in shares: one for the counting kernel, two
+  // for each (longer) scatter kernel. Its last bytes are cleared by themselves.
+  const long words = (long)(dw.numel() * dw.element_size() / 16);
+  const int shares = 1 + 2 * passes;
+  auto share = [&](int from, int to) {
+    const long a = words * from / shares, b = words * to / shares;
+    return Fill{(uint4*)dw.data_ptr() + a, b - a, nblk};
+  };
+  auto blocks = [&](const Fill& f) {  // four stores a thread and no more than
+    return dim3(nblk + (unsigned)std::min<long>((f.n + 1023) / 1024, 4096));
+  };
+  if (dw.numel() * dw.element_size() % 16 != 0) dw.flatten().slice(0, words * 16 / dw.element_size()).zero_();
   DISPATCH_IDS(ids, {
     const id_t* ip = (const id_t*)ids.data_ptr();
-    hipLaunchKernelGGL((sort_count_kernel<id_t>), dim3(nblk), dim3(EMB_BLOCK),
-                       0, stream, ip, (int)N, V, tile, cp, passes - 1);
+    const Fill f0 = share(0, 1);
+    hipLaunchKernelGGL((sort_count_kernel<id_t>), blocks(f0), dim3(EMB_BLOCK),
+                       0, stream, ip, (int)N, V, rounds, cp, passes - 1, f0);
     for (int p = 0; p < passes; ++p) {
       unsigned* in = sp + (long)(1 - at_pair) * 2 * N;
       unsigned* to = sp + (long)at_pair * 2 * N;
       unsigned* c = cp + (long)p * nblk * DIGITS;
       unsigned* next = p + 1 < passes ? c + (long)nblk * DIGITS : nullptr;
-      if (p == 0)
-        hipLaunchKernelGGL((sort_scatter_kernel<id_t, true>), dim3(nblk),
-                           dim3(EMB_BLOCK), 0, stream, ip, in, in + N, to,
-                           to + N, (int)N, V, tile, 8 * p, c, next);
-      else
-        hipLaunchKernelGGL((sort_scatter_kernel<id_t, false>), dim3(nblk),
-                           dim3(EMB_BLOCK), 0, stream, ip, in, in + N, to,
-                           to + N, (int)N, V, tile, 8 * p, c, next);
+      const Fill f = share(1 + 2 * p, 3 + 2 * p);
+      auto scatter = p == 0 ? sort_scatter_kernel<id_t, true>
+                            : sort_scatter_kernel<id_t, false>;
+      hipLaunchKernelGGL(scatter, blocks(f), dim3(EMB_BLOCK), 0, stream, ip,
+                         in, in + N, to, to + N, (int)N, V, rounds, 8 * p, c,
+                         next, f);
       at_pair = 1 - at_pair;
     }
   });
@@ -494,20 +527,19 @@ torch::Tensor embedding_bwd(const torch::Tensor& dy_in,
   const int cols = WAVE * (wide ? 4 : 1);
   const long items = chunks * ((D + cols - 1) / cols);
   const long sum_blocks = (items + SORT_WAVES - 1) / SORT_WAVES;
-  const long fill_rows = SORT_WAVES * FILL_ROWS;
-  const long grid = sum_blocks + (V + fill_rows - 1) / fill_rows;
-  TORCH_CHECK(grid < MAX_GRID && chunks < MAX_GRID,
+  const long col_tiles = (D + cols - 1) / cols;
+  TORCH_CHECK(sum_blocks < MAX_GRID && chunks < MAX_GRID && col_tiles < 65536,
               "embedding: gradient too large");
   DISPATCH_TWO(dy.scalar_type(), w_dtype, {
     auto sum = wide ? embed_sum_kernel<a_t, b_t, 4> : embed_sum_kernel<a_t, b_t, 1>;
-    hipLaunchKernelGGL(sum, dim3(grid), dim3(EMB_BLOCK), 0, stream,
+    hipLaunchKernelGGL(sum, dim3(sum_blocks), dim3(EMB_BLOCK), 0, stream,
                        (const a_t*)dy.data_ptr(), keys, pos,
                        (b_t*)dw.data_ptr(), head, tail, (int)N, D, V,
-                       (float)scale, (int)sum_blocks);
+                       (float)scale);
     auto join = wide ? embed_join_kernel<b_t, 4> : embed_join_kernel<b_t, 1>;
     if (chunks > 1)
-      hipLaunchKernelGGL(join, dim3(chunks - 1), dim3(EMB_BLOCK), 0, stream,
-                         keys, head, tail, (b_t*)dw.data_ptr(), (int)N, D, V,
+      hipLaunchKernelGGL(join, dim3(chunks - 1, col_tiles), dim3(EMB_BLOCK), 0,
+                         stream, keys, head, tail, (b_t*)dw.data_ptr(), (int)N, D, V,
                          (float)scale);
   });
   return dw;
