@@ -33,13 +33,13 @@ def embedding(
     Differentiable once in ``table``. An id outside [0, V) raises IndexError
     on the CPU; on the GPU, where looking would wait for the device, its row
     is NaN and it has no gradient."""
+    out_dtype = out_dtype or table.dtype
+    if use_hip(table):  # checks the same
+        return hip_ext().embedding(ids, table, scale, out_dtype)
     if ids.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"embedding: ids must be int64 or int32, got {ids.dtype}")
     if table.dim() != 2:
         raise ValueError(f"embedding: table must be [V, D], got {tuple(table.shape)}")
-    out_dtype = out_dtype or table.dtype
-    if use_hip(table):
-        return hip_ext().embedding(ids, table, float(scale), out_dtype)
     y = F.embedding(ids, table)
     if scale != 1.0:
         y = y.float() * scale

@@ -600,16 +600,19 @@ bool known_dtype(at::ScalarType t) {
 
 torch::Tensor embedding(torch::Tensor ids, torch::Tensor w, double scale,
                         at::ScalarType out_dtype) {
-  TORCH_CHECK(w.dim() == 2 && w.is_cuda() && known_dtype(w.scalar_type()),
-              "embedding: the table must be a 2D fp32 or bf16 GPU tensor");
+  TORCH_CHECK_TYPE(ids.scalar_type() == at::kLong ||
+                       ids.scalar_type() == at::kInt,
+                   "embedding: ids must be int64 or int32, got ", ids.dtype());
+  TORCH_CHECK_VALUE(w.dim() == 2, "embedding: table must be [V, D], got ",
+                    w.sizes());
+  TORCH_CHECK(w.is_cuda() && known_dtype(w.scalar_type()),
+              "embedding: the table must be fp32 or bf16 on a GPU");
   TORCH_CHECK(w.size(1) < (1L << 30) && w.size(0) < (1L << 31),
               "embedding: table too large");
   TORCH_CHECK(w.size(1) <= 1 || w.stride(1) == 1,
               "embedding: a table row must be contiguous");
   TORCH_CHECK(ids.device() == w.device(), "embedding: ids on ", ids.device(),
               ", table on ", w.device());
-  TORCH_CHECK(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt,
-              "embedding: ids must be int64 or int32");
   TORCH_CHECK(known_dtype(out_dtype), "embedding: output must be fp32 or bf16");
   if (w.requires_grad() && at::GradMode::is_enabled())
     return EmbeddingFn::apply(w, ids, scale, (int64_t)out_dtype);

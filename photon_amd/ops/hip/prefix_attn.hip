@@ -13,30 +13,39 @@ namespace {
 // How a call is cut into workgroups: items of `rows` query rows of one head,
 // the last `rest` of them split `splits` times along the keys.
 struct Cut {
-  int waves;  // of 32 rows each
+  bool few;  // few rows: waves share the keys, not the rows
   int rows, items, full, rest, splits;
   int groups() const { return full + rest * splits; }
   long partial_rows() const { return (long)rest * splits * rows; }
 };
 
+template <int D>
+using FewRows = Shape<D, 1, 4, 2>;
+template <int D>
+using ManyRows = Shape<D, 4, 1, 2>;
+// Few rows are 128 items of 32 rows at most: half the chip, so that the keys
+// can be split at least once more. 16 heads of 128 over 1507 keys, 160 rows (80
+// items): 17 us, and 25 with tiles of 128 rows; 32 heads over 3900 keys, 160
+// rows (160 items): 54 us, and 36.
+constexpr long FEW_ITEMS = 128;
+
 // Whole rounds of items fill the chip by themselves; what is left over is
-// split until it does, but not below two key tiles each. `always`: every item
-// leaves partial rows.
-Cut cut(long T, int H, int D, int key_tiles, bool always) {
+// split until it does, but not below two key tiles (one a wave with few rows)
+// each. `always`: every item leaves partial rows.
+Cut cut(long T, int H, int D, long keys, bool always) {
   Cut c;
-  c.waves = T <= 32 ? 1 : T <= 64 ? 2 : 4;
-  c.rows = c.waves * QB;
+  c.few = (T + FewRows<64>::ROWS - 1) / FewRows<64>::ROWS * H <= FEW_ITEMS;
+  c.rows = c.few ? FewRows<64>::ROWS : ManyRows<64>::ROWS;
   const long items = (T + c.rows - 1) / c.rows * H;
   TORCH_CHECK(items < (1L << 22), "prefix attention: too many rows");
   c.items = (int)items;
-  // a CU holds two workgroups of four waves (three with short heads), or one
-  // with four buffers
-  const int at_once = c.waves < 4 ? 256 : D == 64 ? 768 : 512;
+  // workgroups that are on the chip together, by their registers and LDS
+  const int at_once = c.few ? (D == 64 ? 512 : 256) : (D == 64 ? 768 : 512);
   c.full = always ? 0 : c.items / at_once * at_once;
   c.rest = c.items - c.full;
   c.splits = 1;
   if (c.rest > 0 && c.rest < at_once)
-    c.splits = std::max(1, std::min((at_once + c.rest / 2) / c.rest, key_tiles / 2));
+    c.splits = (int)std::max(1L, std::min<long>(at_once / c.rest, keys / 128));
   if (c.splits == 1 && !always) {
     c.full = c.items;
     c.rest = 0;
@@ -56,33 +65,20 @@ void launch(const torch::Tensor& qkv, const torch::Tensor& prefix, int H,
   cur_stream(), (const __bf16*)qkv.data_ptr(), qkv.stride(0), pk, pv,        \
       prefix.stride(0), slopes.data_ptr<float>(), info.data_ptr<int>(), out, \
       part_o, part_ml, T, P, H, c.full, c.splits
-#define LAUNCH(DD, NW, BUFS)                                                 \
-  hipLaunchKernelGGL((prefix_attn_kernel<DD, NW, BUFS, DECODE>),             \
-                     dim3(c.groups()), dim3(64 * NW),                        \
-                     lds_bytes(DD, NW, BUFS), ARGS)
-#define LAUNCH_D(DD)                                                         \
-  if (c.waves == 1) { LAUNCH(DD, 1, 4); }                                    \
-  else if (c.waves == 2) { LAUNCH(DD, 2, 4); }                               \
-  else if (c.groups() <= 256) { LAUNCH(DD, 4, 4); }                          \
-  else { LAUNCH(DD, 4, 2); }
+#define LAUNCH(SHAPE)                                                        \
+  hipLaunchKernelGGL((prefix_attn_kernel<SHAPE, DECODE>), dim3(c.groups()),  \
+                     dim3(SHAPE::THREADS), SHAPE::BYTES, ARGS)
   if (D == 64) {
-    LAUNCH_D(64)
+    if (c.few) { LAUNCH(FewRows<64>); } else { LAUNCH(ManyRows<64>); }
   } else {
-    LAUNCH_D(128)
+    if (c.few) { LAUNCH(FewRows<128>); } else { LAUNCH(ManyRows<128>); }
   }
-#undef LAUNCH_D
 #undef LAUNCH
 #undef ARGS
 }
 
 // Rows of [q | k | v], 16-byte accesses allowed.
-torch::Tensor checked_rows(const torch::Tensor& t, long width,
-                           const torch::Device& dev, const char* what) {
-  TORCH_CHECK(t.device() == dev && t.scalar_type() == at::kBFloat16,
-              "prefix attention: ", what, " must be bf16 on ", dev);
-  TORCH_CHECK(t.dim() == 2 && t.size(1) == width, "prefix attention: ", what,
-              " must be [rows, ", width, "], got ", t.sizes());
-  TORCH_CHECK(t.size(0) < (1L << 30), "prefix attention: too many rows");
+torch::Tensor rows_of(const torch::Tensor& t, long width) {
   // a tile of 64 rows is addressed with 32-bit byte offsets
   const bool fits = t.size(0) <= 1 || (t.stride(0) >= width &&
                                        t.stride(0) < (1L << 23) &&
@@ -96,59 +92,87 @@ struct Args {
   int T, P, H, D;
 };
 
-Args check(const torch::Tensor& qkv, const torch::Tensor& prefix, long H,
-           const torch::Tensor& slopes, const torch::Tensor& info) {
-  TORCH_CHECK(qkv.is_cuda() && qkv.dim() == 2 && H > 0 && H < 65536 &&
-                  qkv.size(1) % (3 * H) == 0,
-              "prefix attention: qkv must be a GPU tensor [rows, 3 * heads * d]");
-  const long D = qkv.size(1) / (3 * H);
-  TORCH_CHECK(D == 64 || D == 128,
-              "prefix attention: d_head must be 64 or 128, got ", D);
-  TORCH_CHECK(qkv.size(1) < (1L << 23), "prefix attention: rows too long");
+Args check(const char* name, const torch::Tensor& qkv,
+           const torch::Tensor& prefix, long H, const torch::Tensor& slopes,
+           const torch::Tensor& info, const char* info_name) {
+  TORCH_CHECK(!at::GradMode::is_enabled() ||
+                  !(qkv.requires_grad() || prefix.requires_grad() ||
+                    slopes.requires_grad()),
+              name, ": no backward pass; call it under torch.no_grad()");
+  TORCH_CHECK_VALUE(H > 0 && H < 65536 && qkv.dim() == 2 &&
+                        qkv.size(1) % (3 * H) == 0,
+                    name, ": qkv must be [rows, 3 * n_heads * d], got ",
+                    qkv.sizes(), " for ", H, " heads");
+  const long width = qkv.size(1), D = width / (3 * H);
+  TORCH_CHECK_VALUE(prefix.dim() == 2 && prefix.size(1) == width, name,
+                    ": prefix_qkv must be [P, ", width, "], got ",
+                    prefix.sizes());
   const auto dev = qkv.device();
+  TORCH_CHECK_VALUE(prefix.scalar_type() == qkv.scalar_type() &&
+                        prefix.device() == dev,
+                    name, ": prefix_qkv must have qkv's dtype and device");
+  TORCH_CHECK_VALUE(slopes.dim() == 1 && slopes.size(0) == H, name,
+                    ": slopes must be [", H, "], got ", slopes.sizes());
+  TORCH_CHECK_VALUE(info.scalar_type() == at::kInt && info.dim() == 1 &&
+                        info.size(0) == qkv.size(0),
+                    name, ": ", info_name, " must be int32 [", qkv.size(0),
+                    "], got ", info.dtype(), " ", info.sizes());
+  TORCH_CHECK_VALUE(info.device() == dev, name, ": ", info_name,
+                    " must be on ", dev);
+  TORCH_CHECK(qkv.is_cuda() && qkv.scalar_type() == at::kBFloat16, name,
+              ": qkv must be bf16 on a GPU (impl=\"torch\" takes others)");
+  TORCH_CHECK(D == 64 || D == 128, name, ": d_head must be 64 or 128, got ", D);
+  TORCH_CHECK(qkv.size(0) < (1L << 30) && prefix.size(0) < (1L << 30) &&
+                  width < (1L << 23),
+              name, ": too many rows, or too long ones");
   Args a;
-  a.qkv = checked_rows(qkv, qkv.size(1), dev, "qkv");
-  a.prefix = checked_rows(prefix, qkv.size(1), dev, "prefix");
+  a.qkv = rows_of(qkv, width);
+  a.prefix = rows_of(prefix, width);
   a.T = (int)qkv.size(0);
   a.P = (int)prefix.size(0);
   a.H = (int)H;
   a.D = (int)D;
-  TORCH_CHECK(slopes.dim() == 1 && slopes.size(0) == H,
-              "prefix attention: one slope for each head");
-  a.slopes = slopes.to(dev, at::kFloat).contiguous();
-  TORCH_CHECK(info.device() == dev && info.scalar_type() == at::kInt &&
-                  info.dim() == 1 && info.size(0) == a.T,
-              "prefix attention: one int32 for each row of qkv, on its device");
+  a.slopes = slopes.device() == dev && slopes.scalar_type() == at::kFloat
+                 ? slopes.contiguous()
+                 : slopes.to(dev, at::kFloat).contiguous();
   a.info = info.contiguous();
   return a;
 }
+
+// The splits' partial rows, and behind them their maxima and sums.
+struct Partial {
+  torch::Tensor t;
+  float *o = nullptr, *ml = nullptr;
+  Partial() = default;
+  Partial(const Cut& c, int D, const torch::Tensor& like) {
+    if (c.rest == 0) return;
+    t = torch::empty({c.partial_rows() * (D + 2)},
+                     like.options().dtype(at::kFloat));
+    o = t.data_ptr<float>();
+    ml = o + c.partial_rows() * D;
+  }
+};
 
 }  // namespace
 
 torch::Tensor prefix_attention(torch::Tensor qkv, torch::Tensor prefix, long H,
                                torch::Tensor slopes, torch::Tensor starts) {
   const c10::DeviceGuard guard(qkv.device());
-  const Args a = check(qkv, prefix, H, slopes, starts);
+  const Args a = check("prefix_attention_qkv", qkv, prefix, H, slopes, starts,
+                       "starts");
   auto out = torch::empty({(long)a.T, (long)a.H * a.D}, qkv.options());
   if (a.T == 0) return out;
-  const Cut c = cut(a.T, a.H, a.D, (a.P + PKB - 1) / PKB + 1, false);
-  torch::Tensor po, pm;
-  if (c.rest) {
-    auto f = qkv.options().dtype(at::kFloat);
-    po = torch::empty({c.partial_rows() * a.D}, f);
-    pm = torch::empty({c.partial_rows() * 2}, f);
-  }
+  const Cut c = cut(a.T, a.H, a.D, (long)a.P + 64, false);
+  const Partial part(c, a.D, qkv);
   launch<false>(a.qkv, a.prefix, a.H, a.D, a.slopes, a.info,
-                (__bf16*)out.data_ptr(),
-                c.rest ? po.data_ptr<float>() : nullptr,
-                c.rest ? pm.data_ptr<float>() : nullptr, a.T, a.P, c);
+                (__bf16*)out.data_ptr(), part.o, part.ml, a.T, a.P, c);
   if (c.rest) {
     const long threads = (long)c.rest * c.rows * a.D / 4;
     auto join = a.D == 64 ? prefix_join_kernel<64> : prefix_join_kernel<128>;
     hipLaunchKernelGGL(join, dim3((unsigned)((threads + 255) / 256)),
-                       dim3(256), 0, cur_stream(), po.data_ptr<float>(),
-                       pm.data_ptr<float>(), (__bf16*)out.data_ptr(), a.T, a.H,
-                       c.rows, c.full, c.rest, c.splits);
+                       dim3(256), 0, cur_stream(), part.o, part.ml,
+                       (__bf16*)out.data_ptr(), a.T, a.H, c.rows, c.full,
+                       c.rest, c.splits);
   }
   return out;
 }
@@ -156,54 +180,45 @@ torch::Tensor prefix_attention(torch::Tensor qkv, torch::Tensor prefix, long H,
 torch::Tensor prefix_attention_decode(torch::Tensor qkv, torch::Tensor prefix,
                                       long H, torch::Tensor slopes,
                                       torch::Tensor cache, torch::Tensor held) {
+  const char* name = "prefix_attention_decode";
   const c10::DeviceGuard guard(qkv.device());
-  const Args a = check(qkv, prefix, H, slopes, held);
+  const Args a = check(name, qkv, prefix, H, slopes, held, "held");
   const long B = a.T;
-  TORCH_CHECK(cache.device() == qkv.device() &&
-                  cache.scalar_type() == at::kBFloat16 && cache.dim() == 5 &&
-                  cache.size(0) == B && cache.size(2) == 2 &&
-                  cache.size(3) == H && cache.size(4) == a.D,
-              "prefix attention: cache must be bf16 [", B, ", slots, 2, ", H,
-              ", ", a.D, "], got ", cache.sizes());
-  TORCH_CHECK(cache.size(1) < (1L << 30), "prefix attention: too many slots");
+  TORCH_CHECK_VALUE(cache.dim() == 5 && cache.size(0) == B &&
+                        cache.size(2) == 2 && cache.size(3) == H &&
+                        cache.size(4) == a.D,
+                    name, ": cache must be [", B, ", slots, 2, ", H, ", ", a.D,
+                    "], got ", cache.sizes());
+  TORCH_CHECK_VALUE(cache.scalar_type() == qkv.scalar_type() &&
+                        cache.device() == qkv.device(),
+                    name, ": cache must have qkv's dtype and device");
   bool fits = cache.stride(4) == 1 && ((uintptr_t)cache.data_ptr() % 16) == 0;
   for (int d = 0; d < 4; ++d)
     fits = fits && cache.stride(d) % 8 == 0 &&
            (cache.size(d) <= 1 || cache.stride(d) != 0);
-  TORCH_CHECK(fits,
-              "prefix attention: the cache's last dimension must be contiguous "
-              "and its rows aligned to 16 bytes");
-  TORCH_CHECK(B < 65536, "prefix attention: too many sequences");
+  TORCH_CHECK(fits, name,
+              ": the cache's last dimension must be contiguous and its rows "
+              "aligned to 16 bytes");
+  TORCH_CHECK(B < 65536 && cache.size(1) < (1L << 30), name,
+              ": too many sequences or slots");
   auto out = torch::empty({B, (long)a.H * a.D}, qkv.options());
   if (B == 0) return out;
   Cut c{};
-  torch::Tensor po, pm;
-  if (a.P > 0) {
-    c = cut(B, a.H, a.D, (a.P + PKB - 1) / PKB, true);
-    auto f = qkv.options().dtype(at::kFloat);
-    po = torch::empty({c.partial_rows() * a.D}, f);
-    pm = torch::empty({c.partial_rows() * 2}, f);
-    launch<true>(a.qkv, a.prefix, a.H, a.D, a.slopes, a.info, nullptr,
-                 po.data_ptr<float>(), pm.data_ptr<float>(), a.T, a.P, c);
-  }
-  const dim3 grid(a.H, (unsigned)B);
-  const float* pop = c.splits ? po.data_ptr<float>() : nullptr;
-  const float* pmp = c.splits ? pm.data_ptr<float>() : nullptr;
-#define LAUNCH_OWN(DD)                                                        \
-  hipLaunchKernelGGL((decode_own_kernel<DD>), grid, dim3(OWN_BLOCK), 0,       \
-                     cur_stream(), (const __bf16*)a.qkv.data_ptr(),           \
-                     a.qkv.stride(0), (__bf16*)cache.data_ptr(),              \
-                     cache.stride(0), cache.stride(1), cache.stride(2),       \
-                     cache.stride(3), a.slopes.data_ptr<float>(),             \
-                     a.info.data_ptr<int>(), pop, pmp,                        \
-                     (__bf16*)out.data_ptr(), a.H, (int)cache.size(1),        \
-                     std::max(1, c.rows), c.items, c.splits)
-  if (a.D == 64) {
-    LAUNCH_OWN(64);
-  } else {
-    LAUNCH_OWN(128);
-  }
-#undef LAUNCH_OWN
+  c.rows = 1;
+  if (a.P > 0) c = cut(B, a.H, a.D, a.P, true);
+  const Partial part(c, a.D, qkv);
+  if (a.P > 0)
+    launch<true>(a.qkv, a.prefix, a.H, a.D, a.slopes, a.info, nullptr, part.o,
+                 part.ml, a.T, a.P, c);
+  auto own = a.D == 64 ? decode_own_kernel<64> : decode_own_kernel<128>;
+  hipLaunchKernelGGL(own, dim3(a.H, (unsigned)B), dim3(OWN_BLOCK), 0,
+                     cur_stream(), (const __bf16*)a.qkv.data_ptr(),
+                     a.qkv.stride(0), (__bf16*)cache.data_ptr(),
+                     cache.stride(0), cache.stride(1), cache.stride(2),
+                     cache.stride(3), a.slopes.data_ptr<float>(),
+                     a.info.data_ptr<int>(), part.o, part.ml,
+                     (__bf16*)out.data_ptr(), a.H, (int)cache.size(1), c.rows,
+                     c.items, c.splits);
   return out;
 }
 

@@ -24,7 +24,25 @@
 
 namespace photon_hip {
 
-constexpr int PKB = 64;  // keys a tile
+// A workgroup is NW x KW waves: NW of 32 query rows each that share their key
+// tiles (64 keys), or, where there are few rows, KW that take every KW-th key
+// tile (32 keys) of the same rows and are joined at the end. BUFS tiles are in
+// LDS or on their way for each.
+template <int D_, int NW_, int KW_, int BUFS_>
+struct Shape {
+  static constexpr int D = D_, NW = NW_, KW = KW_, BUFS = BUFS_;
+  static constexpr int SUBS = KW == 1 ? 2 : 1;  // subtiles of 32 keys
+  static constexpr int KEYS = 32 * SUBS;
+  static constexpr int IMG = KEYS * D * 2;      // bytes of a [KEYS][D] image
+  static constexpr int THREADS = 64 * NW * KW;
+  static constexpr int ROWS = 32 * NW;
+  // LDS: the images (or, at the end, the waves' fp32 rows), then each wave's
+  // maxima and sums; a word a wave for the search of bad values
+  static constexpr int IMAGES = KW * BUFS * 2 * IMG;
+  static constexpr int FP32_ROWS = NW * KW * 32 * D * 4;
+  static constexpr int STATS = IMAGES > FP32_ROWS ? IMAGES : FP32_ROWS;
+  static constexpr int BYTES = STATS + NW * KW * 32 * 8;
+};
 
 // Buffer descriptor of `bytes` from `base` as four words (flags: a valid
 // format, see make_rsrc), and a copy of 16 bytes a lane to LDS through it.
@@ -61,6 +79,11 @@ DEV_INLINE void vm_wait() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// Until this wave's LDS accesses are done.
+DEV_INLINE void lds_wait0() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
 // The larger of a row's two halves (lanes l and l + 32); NaN if one is.
 DEV_INLINE float swap_max(float x) {
   union { float f; unsigned u; } a, b;
@@ -91,39 +114,27 @@ DEV_INLINE bf16x8 pack_weights(const float* p) {
   return out.v;
 }
 
-// LDS: `bufs` buffers of a key and a value image (or, at the end, the fp32
-// rows of all waves), and a word for each wave.
-constexpr int lds_images(int D, int nw, int bufs) {
-  const int images = bufs * 2 * PKB * D * 2, rows = nw * 32 * D * 4;
-  return images > rows ? images : rows;
-}
-constexpr int lds_bytes(int D, int nw, int bufs) {
-  return lds_images(D, nw, bufs) + 64;
-}
-
 // Swapped product (keys x queries): lane holds query lane & 31, its 16
 // registers the keys (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5) of 32.
 //
 // `info` is each row's first own row (packed form) or, in the decode form, how
 // many own keys the row's sequence holds; there the kernel covers the prefix
 // only.
-//
-// BUFS key tiles are in LDS or on their way. Two, and two workgroups a CU,
-// where there are many; four where a CU has one at most and nothing else hides
-// the way from memory.
-template <int D, int NW, int BUFS, bool DECODE>
-__global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void prefix_attn_kernel(
+template <typename S, bool DECODE>
+__global__ __launch_bounds__(S::THREADS, S::D == 64 ? 3 : 2) void prefix_attn_kernel(
     const __bf16* __restrict__ qkv, long q_rs, const __bf16* __restrict__ pk,
     const __bf16* __restrict__ pv, long p_rs,
     const float* __restrict__ slopes, const int* __restrict__ info,
     __bf16* __restrict__ out, float* __restrict__ part_o,
     float* __restrict__ part_ml, int T, int P, int H, int full, int splits) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int IMG = PKB * D * 2;  // bytes of a [64][D] image
+  constexpr int D = S::D, NW = S::NW, KW = S::KW, BUFS = S::BUFS;
+  constexpr int SUBS = S::SUBS, KEYS = S::KEYS, IMG = S::IMG;
   constexpr bool D64 = D == 64;
 
   const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rw = wave % NW, kw = wave / NW;  // rows, keys of this wave
   const int hi = lane >> 5;
   const int lq = lane & 31;
   // the first `full` items (query tile, head) are whole, the others split
@@ -135,22 +146,14 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void prefix_attn_kernel(
   }
   const int h = item % H;
   const int q0_block = item / H * (NW * QB);
-  const int my_q = q0_block + wave * QB + lq;
+  const int my_q = q0_block + rw * QB + lq;
   const int row = min(my_q, T - 1);
-
-  const float scale2 = rsqrtf((float)D) * LOG2E;
-  const float slope2 = slopes[h] * LOG2E;
 
   const __bf16* q = qkv + (long)h * D;
   const __bf16* k = q + (long)H * D;
   const __bf16* v = k + (long)H * D;
   pk += (long)h * D;
   pv += (long)h * D;
-
-  bf16x8 qfrag[D / 16];
-#pragma unroll
-  for (int kk = 0; kk < D / 16; ++kk)
-    qfrag[kk] = *(const bf16x8*)(q + row * q_rs + kk * 16 + 8 * hi);
 
   // own position of this lane's row, and the first packed row it may see
   int first = 0, own = 0;
@@ -162,18 +165,73 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void prefix_attn_kernel(
   }
 
   // key tiles: the prefix's, then the packed rows lo..hi_row of this block
-  const int n_pre = (P + PKB - 1) / PKB;
+  const int n_pre = (P + KEYS - 1) / KEYS;
   int lo = 0, n_own = 0, end_row = 0;
   if (!DECODE) {
     lo = __builtin_amdgcn_readfirstlane(
         min(max(info[q0_block], 0), q0_block));
     end_row = min(q0_block + NW * QB, T);
-    n_own = (end_row - lo + PKB - 1) / PKB;
+    n_own = (end_row - lo + KEYS - 1) / KEYS;
   }
   const int n_all = n_pre + n_own;
   const int each = n_all / parts, more = n_all - each * parts;
   const int t0 = split * each + min(split, more);
   const int t1 = t0 + each + (split < more ? 1 : 0);
+
+  // Staging: a wave-instruction moves 1 KiB to LDS, lane by lane in order;
+  // the swizzle is applied to the source. The descriptor starts at the tile
+  // (64-bit base), so a prefix of any length keeps 32-bit offsets, and ends
+  // with its last row: what lies behind reads as zeros.
+  constexpr int NWIN = IMG / 1024 / NW;
+  int dma_row[NWIN], dma_col[NWIN];
+#pragma unroll
+  for (int i = 0; i < NWIN; ++i) {
+    const int dest = (rw * NWIN + i) * 1024 + lane * 16;
+    const int r = dest / (D * 2);
+    dma_row[i] = r;
+    dma_col[i] =
+        (dest ^ (int)(swz_field((unsigned)r & 15u, D64) << 4)) % (D * 2);
+  }
+  char* const images = smem + kw * (BUFS * 2 * IMG);
+  const unsigned wave_win = __builtin_amdgcn_readfirstlane(
+      lds_base(smem) + kw * (BUFS * 2 * IMG) + rw * (NWIN * 1024));
+  auto stage = [&](int t, int b) {
+    const bool pre = t < n_pre;
+    const long rs = pre ? p_rs : q_rs;
+    const long at = pre ? (long)t * KEYS : (long)lo + (long)(t - n_pre) * KEYS;
+    const int rows = min(KEYS, (pre ? P : end_row) - (int)at);
+    const long bytes = ((long)(rows - 1) * rs + D) * 2;
+    const desc_t krs = make_desc((pre ? pk : k) + at * rs, bytes);
+    const desc_t vrs = make_desc((pre ? pv : v) + at * rs, bytes);
+    const int rs2 = (int)(rs * 2);
+    const unsigned dst = wave_win + b * 2 * IMG;
+#pragma unroll
+    for (int i = 0; i < NWIN; ++i) {
+      const int off = dma_row[i] * rs2 + dma_col[i];
+      copy16_to_lds(krs, dst + i * 1024, off);
+      copy16_to_lds(vrs, dst + IMG + i * 1024, off);
+    }
+  };
+
+  // From the nearest keys to the farthest: ALiBi makes the weights fall on
+  // the way, so the first tiles set the maximum and the sums are hardly ever
+  // rescaled (forwards, a steep head's maximum rises with every tile). With
+  // few rows, where the whole call is one chain of latencies, the first copies
+  // leave before anything else is loaded.
+  const int last = t1 - 1 - kw;
+  auto first_copies = [&]() {
+#pragma unroll
+    for (int i = 0; i < BUFS - 1; ++i)
+      if (last - i * KW >= t0) stage(last - i * KW, i);
+  };
+  if constexpr (KW > 1) first_copies();
+
+  const float scale2 = rsqrtf((float)D) * LOG2E;
+  const float slope2 = slopes[h] * LOG2E;
+  bf16x8 qfrag[D / 16];
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk)
+    qfrag[kk] = *(const bf16x8*)(q + row * q_rs + kk * 16 + 8 * hi);
 
   float m_run = -1e30f;  // finite: exp2(-huge) == 0 and no NaN from inf - inf
   float l_run = 0.f;      // this half's share of the sum
@@ -189,40 +247,6 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void prefix_attn_kernel(
   for (int r = 0; r < 16; ++r)
     alibi[r] = slopes[h] * sqrtf((float)D) *
                (float)((r & 3) + 8 * (r >> 2) + 4 * hi);
-
-  // Staging: a wave-instruction moves 1 KiB to LDS, lane by lane in order;
-  // the swizzle is applied to the source. The descriptor starts at the tile
-  // (64-bit base), so a prefix of any length keeps 32-bit offsets, and ends
-  // with its last row: what lies behind reads as zeros.
-  constexpr int NWIN = IMG / 1024 / NW;
-  int dma_row[NWIN], dma_col[NWIN];
-#pragma unroll
-  for (int i = 0; i < NWIN; ++i) {
-    const int dest = (wave * NWIN + i) * 1024 + lane * 16;
-    const int r = dest / (D * 2);
-    dma_row[i] = r;
-    dma_col[i] =
-        (dest ^ (int)(swz_field((unsigned)r & 15u, D64) << 4)) % (D * 2);
-  }
-  const unsigned wave_win =
-      lds_base(smem) + __builtin_amdgcn_readfirstlane(wave) * (NWIN * 1024);
-  auto stage = [&](int t, int b) {
-    const bool pre = t < n_pre;
-    const long rs = pre ? p_rs : q_rs;
-    const long at = pre ? (long)t * PKB : (long)lo + (long)(t - n_pre) * PKB;
-    const int rows = min(PKB, (pre ? P : end_row) - (int)at);
-    const long bytes = ((long)(rows - 1) * rs + D) * 2;
-    const desc_t krs = make_desc((pre ? pk : k) + at * rs, bytes);
-    const desc_t vrs = make_desc((pre ? pv : v) + at * rs, bytes);
-    const int rs2 = (int)(rs * 2);
-    const unsigned dst = wave_win + b * 2 * IMG;
-#pragma unroll
-    for (int i = 0; i < NWIN; ++i) {
-      const int off = dma_row[i] * rs2 + dma_col[i];
-      copy16_to_lds(krs, dst + i * 1024, off);
-      copy16_to_lds(vrs, dst + IMG + i * 1024, off);
-    }
-  };
 
   // LDS read addresses (see the swizzle's row rule in attn_kernels.h)
   unsigned qk_addr[D / 16];
@@ -241,26 +265,26 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void prefix_attn_kernel(
       pv_addr[rd][db] = swz((unsigned)(key0 * (D * 2) + dh * 2), key0, D64);
     }
   }
-  // Both subtiles' scores. All fragments are read before the products: left
-  // to itself the compiler reads each into the same registers and waits.
-  auto scores = [&](int b, f32x16 (&s)[2]) {
-    bf16x8 a[2][D / 16];
+  // The tile's scores. All fragments are read before the products: left to
+  // itself the compiler reads each into the same registers and waits.
+  auto scores = [&](int b, f32x16 (&s)[SUBS]) {
+    bf16x8 a[SUBS][D / 16];
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
+    for (int sub = 0; sub < SUBS; ++sub)
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk)
-        a[sub][kk] = *(const bf16x8*)(smem + qk_addr[kk] + b * 2 * IMG +
+        a[sub][kk] = *(const bf16x8*)(images + qk_addr[kk] + b * 2 * IMG +
                                       sub * 32 * (D * 2));
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
+    for (int sub = 0; sub < SUBS; ++sub) {
       s[sub] = alibi;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk)
         s[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[sub][kk], qfrag[kk],
                                                          s[sub], 0, 0, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x100, D / 8, 0);  // LDS reads
-    __builtin_amdgcn_sched_group_barrier(0x008, D / 8, 0);  // products
+    __builtin_amdgcn_sched_group_barrier(0x100, SUBS * D / 16, 0);  // LDS reads
+    __builtin_amdgcn_sched_group_barrier(0x008, SUBS * D / 16, 0);  // products
   };
   auto add_values = [&](const float* p, int b, int sub) {
 #pragma unroll
@@ -271,7 +295,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void prefix_attn_kernel(
         union { bf16x4 half[2]; bf16x8 all; } a;
 #pragma unroll
         for (int rd = 0; rd < 2; ++rd)
-          a.half[rd] = lds_tr16((const __bf16*)(smem + IMG),
+          a.half[rd] = lds_tr16((const __bf16*)(images + IMG),
                                 pv_addr[rd][db] + b * 2 * IMG +
                                     sub * 32 * (D * 2) + s16 * 16 * (D * 2));
         o_acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.all, pf,
@@ -299,40 +323,45 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void prefix_attn_kernel(
   // packed rows a value belongs to other sequences or later rows as well. So
   // values that are not finite are taken out of such a tile (returns whether
   // there were any) and added by add_bad() where they are seen.
-  int* bad_words = (int*)(smem + lds_images(D, NW, BUFS));
+  int* bad_words = (int*)(smem + S::STATS);
   auto take_out_bad = [&](int b) {
-    uint4* img = (uint4*)(smem + b * 2 * IMG + IMG);
-    constexpr int EACH = IMG / 16 / (64 * NW);
+    uint4* img = (uint4*)(images + b * 2 * IMG + IMG);
+    constexpr int STEP = 64 * NW, EACH = IMG / 16 / STEP;
+    const int me = rw * 64 + lane;
     auto bad_half = [](unsigned w, unsigned mask) { return (w & mask) == mask; };
     auto bad_word = [&](unsigned w) {
       return bad_half(w, 0x7f800000u) | bad_half(w, 0x7f80u);
     };
     uint4 w[EACH];
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) w[i] = img[threadIdx.x + i * 64 * NW];
+    for (int i = 0; i < EACH; ++i) w[i] = img[me + i * STEP];
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < EACH; ++i)
       bad |= bad_word(w[i].x) | bad_word(w[i].y) | bad_word(w[i].z) |
              bad_word(w[i].w);
-    const bool wave_bad = __any(bad);
-    if (lane == 0) bad_words[wave] = wave_bad;
-    __syncthreads();
-    bool any = false;
+    bool any = __any(bad);
+    if (KW == 1) {
+      if (lane == 0) bad_words[wave] = any;
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; ++w) any |= bad_words[w] != 0;
+      for (int w = 0; w < NW; ++w) any |= bad_words[w] != 0;
+    }
     if (!any) return false;
     unsigned* words = (unsigned*)img;
 #pragma unroll 1
-    for (int i = threadIdx.x; i < IMG / 4; i += 64 * NW) {
+    for (int i = me; i < IMG / 4; i += STEP) {
       if (bad_half(words[i], 0x7f800000u)) words[i] &= 0xffffu;
       if (bad_half(words[i], 0x7f80u)) words[i] &= 0xffff0000u;
     }
-    __syncthreads();
+    if (KW == 1)
+      __syncthreads();
+    else
+      lds_wait0();
     return true;
   };
   auto add_bad = [&](int kv0) {
-    const int end = min(kv0 + PKB, end_row);
+    const int end = min(kv0 + KEYS, end_row);
 #pragma unroll 1
     for (int key = kv0; key < end; ++key) {
       const bool seen = key >= first && key <= row;
@@ -347,35 +376,37 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void prefix_attn_kernel(
     }
   };
 
-  // From the nearest keys to the farthest: ALiBi makes the weights fall on
-  // the way, so the first tiles set the maximum and the sums are hardly ever
-  // rescaled (forwards, a steep head's maximum rises with every tile).
-#pragma unroll
-  for (int i = 0; i < BUFS - 1; ++i)
-    if (t1 - 1 - i >= t0) stage(t1 - 1 - i, i);
+  // All loads so far (vmcnt 0; a wait that the compiler knows of): otherwise it
+  // waits for the query's inside the loop, and with them for the next tile.
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  if constexpr (KW == 1) first_copies();
   int b = BUFS - 1;
-  for (int t = t1 - 1; t >= t0; --t) {
-    const int old = b;  // the buffer of tile t + 1
+  for (int t = last; t >= t0; t -= KW) {
+    const int old = b;  // the buffer of the tile before
     b = b == BUFS - 1 ? 0 : b + 1;
     // the copies of the BUFS - 2 tiles behind t may still be on their way
-    if (t - t0 >= BUFS - 2)
+    if (t - (BUFS - 2) * KW >= t0)
       vm_wait<(BUFS - 2) * 2 * NWIN < 63 ? (BUFS - 2) * 2 * NWIN : 63>();
     else
       vm_wait0();
-    __syncthreads();  // tile t is there; all reads of tile t + 1 are done
-    if (t - (BUFS - 1) >= t0) stage(t - (BUFS - 1), old);
+    // tile t is there, and the reads of the one before are done
+    if (KW == 1)
+      __syncthreads();
+    else
+      lds_wait0();
+    if (t - (BUFS - 1) * KW >= t0) stage(t - (BUFS - 1) * KW, old);
     const bool pre = t < n_pre;
-    const int kv0 = pre ? t * PKB : lo + (t - n_pre) * PKB;
-    const bool masked = !pre || (t + 1) * PKB > P;
+    const int kv0 = pre ? t * KEYS : lo + (t - n_pre) * KEYS;
+    const bool masked = !pre || (t + 1) * KEYS > P;
     const bool bad = pre ? false : take_out_bad(b);
-    f32x16 s[2];
+    f32x16 s[SUBS];
     scores(b, s);
     if (masked) {
       // keys from .. from + span of this row, counted from the lane's first
       const int from = (pre ? 0 : first) - (kv0 + 4 * hi);
       const unsigned span = pre ? P - 1 : row - first;
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
+      for (int sub = 0; sub < SUBS; ++sub)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int key = sub * 32 + (r & 3) + 8 * (r >> 2);
@@ -383,21 +414,24 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void prefix_attn_kernel(
         }
     }
     const float c = slope2 * (float)(kv0 - (pre ? P + own : row));
-    float x = s[0][0], y = s[1][0];
+    float top[SUBS];
 #pragma unroll
-    for (int r = 1; r < 16; ++r) {
-      x = __builtin_elementwise_maximum(x, s[0][r]);
-      y = __builtin_elementwise_maximum(y, s[1][r]);
+    for (int sub = 0; sub < SUBS; ++sub) {
+      top[sub] = s[sub][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r)
+        top[sub] = __builtin_elementwise_maximum(top[sub], s[sub][r]);
+      top[sub] = fmaf(top[sub], scale2, c + (float)(32 * sub) * slope2);
     }
-    const float top = swap_max(__builtin_elementwise_maximum(
-        fmaf(x, scale2, c), fmaf(y, scale2, c + 32.f * slope2)));
+    const float highest = swap_max(
+        __builtin_elementwise_maximum(top[0], top[SUBS - 1]));
     // Below 2^-150 of the maximum a weight is zero in fp32: a tile of such
     // weights (far keys of a steep head, other sequences' rows) adds nothing.
     // A NaN among the scores makes the comparison false.
-    if (!bad && __all(top - m_run < -150.f)) continue;
-    raise(top);
+    if (!bad && __all(highest - m_run < -150.f)) continue;
+    raise(highest);
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
+    for (int sub = 0; sub < SUBS; ++sub) {
       const float shift = c + (float)(32 * sub) * slope2 - m_run;
       float p[16];
 #pragma unroll
@@ -412,8 +446,12 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void prefix_attn_kernel(
   l_run += __shfl_xor(l_run, 32, 64);
   __syncthreads();  // the images are free
 
-  // Through LDS to whole rows. A wave has the 32 x D values of its own rows.
-  if (parts == 1 && !DECODE) {
+  // Through LDS to whole rows.
+  const int rest = (T + S::ROWS - 1) / S::ROWS * H - full;
+  // partial rows: [split][item - full][row of the item]
+  const long base = ((long)split * rest + item - full) * S::ROWS;
+  const bool whole = parts == 1 && !DECODE;
+  if (KW == 1 && whole) {
     __bf16* o_img = (__bf16*)smem + wave * 32 * D;
     const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
 #pragma unroll
@@ -424,31 +462,72 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void prefix_attn_kernel(
             (__bf16)(o_acc[db][r] * inv);
     __syncthreads();
     for (int c = lane; c < 32 * D / 8; c += 64) {
-      const int r = q0_block + wave * QB + c / (D / 8);
+      const int r = q0_block + rw * QB + c / (D / 8);
       const int col = (c % (D / 8)) * 8;
       if (r < T)
         *(bf16x8*)(out + (long)r * H * D + (long)h * D + col) =
             *(const bf16x8*)(o_img + c * 8);
     }
-  } else {
-    float* o_img = (float*)smem + wave * 32 * D;
+    return;
+  }
+  float* o_img = (float*)smem + wave * 32 * D;
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db)
+  for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-      for (int r = 0; r < 16; r += 4)
-        *(f32x4*)(o_img + lq * D + db * 32 + 2 * r + 4 * hi) =
-            f32x4{o_acc[db][r], o_acc[db][r + 1], o_acc[db][r + 2],
-                  o_acc[db][r + 3]};
+    for (int r = 0; r < 16; r += 4)
+      *(f32x4*)(o_img + lq * D + db * 32 + 2 * r + 4 * hi) =
+          f32x4{o_acc[db][r], o_acc[db][r + 1], o_acc[db][r + 2],
+                o_acc[db][r + 3]};
+  if (KW == 1) {
     __syncthreads();
-    // partial rows: [split][item - full][row of the item]
-    const int rest = (T + NW * QB - 1) / (NW * QB) * H - full;
-    const long base =
-        ((long)split * rest + item - full) * (NW * QB) + wave * QB;
     for (int c = lane; c < 32 * D / 4; c += 64)
-      *(f32x4*)(part_o + base * D + c * 4) = *(const f32x4*)(o_img + c * 4);
+      *(f32x4*)(part_o + (base + rw * QB) * D + c * 4) =
+          *(const f32x4*)(o_img + c * 4);
     if (hi == 0) {
-      part_ml[(base + lq) * 2] = m_run;
-      part_ml[(base + lq) * 2 + 1] = l_run;
+      part_ml[(base + rw * QB + lq) * 2] = m_run;
+      part_ml[(base + rw * QB + lq) * 2 + 1] = l_run;
+    }
+  } else {
+    float* stats = (float*)(smem + S::STATS);  // [wave][row]: maximum, sum
+    if (hi == 0) {
+      stats[(wave * 32 + lq) * 2] = m_run;
+      stats[(wave * 32 + lq) * 2 + 1] = l_run;
+    }
+    __syncthreads();
+    // a row's key waves: EACH threads a row, four columns at a time
+    constexpr int EACH = S::THREADS / 32;
+    const int r = threadIdx.x / EACH;
+    float M = -1e30f, l = 0.f, a[KW];
+#pragma unroll
+    for (int w = 0; w < KW; ++w) M = fmaxf(M, stats[(w * 32 + r) * 2]);
+#pragma unroll
+    for (int w = 0; w < KW; ++w) {
+      a[w] = exp2_fast(stats[(w * 32 + r) * 2] - M);
+      l += a[w] * stats[(w * 32 + r) * 2 + 1];
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const int q_row = q0_block + r;
+    for (int c = (threadIdx.x % EACH) * 4; c < D; c += EACH * 4) {
+      f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const f32x4 x = *(const f32x4*)((float*)smem + (w * 32 + r) * D + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] += a[w] * x[j];
+      }
+      if (whole) {
+        bf16x4 y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = (__bf16)(o[j] * inv);
+        if (q_row < T)
+          *(bf16x4*)(out + (long)q_row * H * D + (long)h * D + c) = y;
+      } else {
+        *(f32x4*)(part_o + (base + r) * D + c) = o;
+      }
+    }
+    if (!whole && threadIdx.x % EACH == 0) {
+      part_ml[(base + r) * 2] = M;
+      part_ml[(base + r) * 2 + 1] = l;
     }
   }
 }
@@ -518,6 +597,22 @@ __global__ __launch_bounds__(OWN_BLOCK) void decode_own_kernel(
   if (n < 0 || n >= slots) {  // no room for the new key: say so
     if (tid < D) o_row[tid] = (__bf16)__builtin_nanf("");
     return;
+  }
+  // The first of the prefix's partial rows are asked for before the sequence's
+  // own keys: their way from memory is not on the chain behind them.
+  constexpr int EARLY = 8;
+  const long stride = (long)items * rows;
+  const long pr = ((long)(b / rows) * H + h) * rows + b % rows;
+  float pm[EARLY], pl[EARLY], po[EARLY];
+#pragma unroll
+  for (int s = 0; s < EARLY; ++s) {
+    pm[s] = -1e30f;
+    pl[s] = po[s] = 0.f;
+    if (s < splits && tid < D) {
+      pm[s] = part_ml[(s * stride + pr) * 2];
+      pl[s] = part_ml[(s * stride + pr) * 2 + 1];
+      po[s] = part_o[(s * stride + pr) * D + tid];
+    }
   }
   __bf16* ck = cache + b * c_bs + (long)h * c_hs;
   __bf16* cv = ck + c_ks;
@@ -600,13 +695,12 @@ __global__ __launch_bounds__(OWN_BLOCK) void decode_own_kernel(
   }
   __syncthreads();
   if (tid >= D) return;
-  // the sequence's row of the prefix's partial ones
-  const long stride = (long)items * rows;
-  const long rh = ((long)(b / rows) * H + h) * rows + b % rows;
   float M = -1e30f;
+#pragma unroll
+  for (int s = 0; s < EARLY; ++s) M = fmaxf(M, pm[s]);
 #pragma unroll 8
-  for (int s = 0; s < splits; ++s)
-    M = fmaxf(M, part_ml[(s * stride + rh) * 2]);
+  for (int s = EARLY; s < splits; ++s)
+    M = fmaxf(M, part_ml[(s * stride + pr) * 2]);
 #pragma unroll
   for (int w = 0; w < OWN_BLOCK / 64; ++w) M = fmaxf(M, s_m[w]);
   float sum = 0.f, acc = 0.f;
@@ -616,11 +710,17 @@ __global__ __launch_bounds__(OWN_BLOCK) void decode_own_kernel(
     sum += a * s_l[w];
     acc += a * s_o[w][tid];
   }
+#pragma unroll
+  for (int s = 0; s < EARLY; ++s) {
+    const float a = exp2_fast(pm[s] - M);
+    sum += a * pl[s];
+    acc += a * po[s];
+  }
 #pragma unroll 8
-  for (int s = 0; s < splits; ++s) {
-    const float a = exp2_fast(part_ml[(s * stride + rh) * 2] - M);
-    sum += a * part_ml[(s * stride + rh) * 2 + 1];
-    acc += a * part_o[(s * stride + rh) * D + tid];
+  for (int s = EARLY; s < splits; ++s) {
+    const float a = exp2_fast(part_ml[(s * stride + pr) * 2] - M);
+    sum += a * part_ml[(s * stride + pr) * 2 + 1];
+    acc += a * part_o[(s * stride + pr) * D + tid];
   }
   o_row[tid] = (__bf16)(acc / sum);
 }

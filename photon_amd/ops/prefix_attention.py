@@ -37,6 +37,7 @@ def sequence_starts(lengths, device=None) -> torch.Tensor:
 
 
 def _check(name, qkv, prefix_qkv, n_heads, slopes, info, info_name):
+    """Of the plain path; the extension checks the same with the same words."""
     if torch.is_grad_enabled() and any(
             t.requires_grad for t in (qkv, prefix_qkv, slopes)):
         raise RuntimeError(f"{name}: no backward pass; call it under torch.no_grad()")
@@ -73,9 +74,9 @@ def prefix_attention_qkv(
 
     impl="flash" on a GPU is the HIP kernel (bf16, d 64 or 128); elsewhere,
     and for impl="torch", plain torch in fp32."""
-    _check("prefix_attention_qkv", qkv, prefix_qkv, n_heads, slopes, starts, "starts")
     if impl == "flash" and use_hip(qkv):
         return hip_ext().prefix_attention(qkv, prefix_qkv, n_heads, slopes, starts)
+    _check("prefix_attention_qkv", qkv, prefix_qkv, n_heads, slopes, starts, "starts")
     return _plain(qkv, prefix_qkv, n_heads, slopes, starts)
 
 
@@ -99,6 +100,9 @@ def prefix_attention_decode(
 
     A sequence without a free slot raises IndexError on the CPU; on the GPU
     its output is NaN and its cache stays."""
+    if impl == "flash" and use_hip(qkv):
+        return hip_ext().prefix_attention_decode(
+            qkv, prefix_qkv, n_heads, slopes, cache, held)
     name = "prefix_attention_decode"
     _check(name, qkv, prefix_qkv, n_heads, slopes, held, "held")
     want = (2, n_heads, qkv.shape[1] // (3 * n_heads))
@@ -107,9 +111,6 @@ def prefix_attention_decode(
                          f"{', '.join(map(str, want))}], got {tuple(cache.shape)}")
     if cache.dtype != qkv.dtype or cache.device != qkv.device:
         raise ValueError(f"{name}: cache must have qkv's dtype and device")
-    if impl == "flash" and use_hip(qkv):
-        return hip_ext().prefix_attention_decode(
-            qkv, prefix_qkv, n_heads, slopes, cache, held)
     B = qkv.shape[0]
     rows, slots = held.long(), cache.shape[1]
     if bool(((rows < 0) | (rows >= slots)).any()):

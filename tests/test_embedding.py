@@ -183,6 +183,10 @@ def test_gpu_refusals(dev):
         embedding(ids, w.half())
     with pytest.raises(RuntimeError, match="fp32 or bf16"):
         embedding(ids, w, 1.0, torch.float16)
+    with pytest.raises(TypeError, match="int64 or int32"):
+        embedding(ids.float(), w)
+    with pytest.raises(ValueError, match=r"\[V, D\]"):
+        embedding(ids, w[0])
     with pytest.raises(RuntimeError, match="ids on"):
         embedding(ids.cpu(), w)
     y = embedding(ids, w)
