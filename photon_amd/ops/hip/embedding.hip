@@ -267,6 +267,117 @@ __global__ __launch_bounds__(EMB_BLOCK) void sort_scatter_kernel(
   }
 }
 
+// Up to ONE_BLOCK_IDS positions: all passes in one workgroup, the items in
+// registers and one exchange through LDS a pass, beside the blocks that clear
+// the gradient. Every launch costs the host 3 to 4 us, and four of them are
+// longer than the sort.
+constexpr int ONE_BLOCK = 1024;
+constexpr int ONE_WAVES = ONE_BLOCK / WAVE;
+constexpr long ONE_BLOCK_IDS = ONE_BLOCK * 16;
+
+template <typename I, int ONE_ITEMS>
+__global__ __launch_bounds__(ONE_BLOCK) void sort_one_block_kernel(
+    const I* __restrict__ ids, unsigned* __restrict__ keys_out,
+    unsigned* __restrict__ pos_out, int N, long V, int passes,
+    const Fill fill) {
+  if ((int)blockIdx.x >= fill.first) {
+    const long step = (long)(gridDim.x - fill.first) * ONE_BLOCK;
+#pragma unroll 4
+    for (long i = (long)(blockIdx.x - fill.first) * ONE_BLOCK + threadIdx.x;
+         i < fill.n; i += step)
+      fill.p[i] = uint4{0, 0, 0, 0};
+    return;
+  }
+  __shared__ unsigned s_key[ONE_BLOCK * ONE_ITEMS];
+  __shared__ unsigned s_pos[ONE_BLOCK * ONE_ITEMS];
+  __shared__ unsigned offs[ONE_WAVES][DIGITS];
+  __shared__ unsigned wave_totals[SORT_WAVES];
+  const int tid = threadIdx.x;
+  const int lane = tid & (WAVE - 1);
+  const int wid = tid / WAVE;
+  const int i0 = wid * (WAVE * ONE_ITEMS) + lane;  // a wave's items are in order
+  unsigned key[ONE_ITEMS], pos[ONE_ITEMS];
+#pragma unroll
+  for (int j = 0; j < ONE_ITEMS; ++j) {
+    const int i = i0 + j * WAVE;
+    key[j] = i < N ? token_key(ids, i, V) : 0u;
+    pos[j] = (unsigned)i;
+  }
+  for (int p = 0; p < passes; ++p) {
+    const int shift = 8 * p;
+    for (int i = tid; i < ONE_WAVES * DIGITS; i += ONE_BLOCK)
+      (&offs[0][0])[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ONE_ITEMS; ++j)
+      if (i0 + j * WAVE < N) atomicAdd(&offs[wid][(key[j] >> shift) & 255u], 1u);
+    __syncthreads();
+    unsigned total = 0, scan = 0;
+    if (tid < DIGITS) {
+#pragma unroll
+      for (int w = 0; w < ONE_WAVES; ++w) total += offs[w][tid];
+      scan = total;
+#pragma unroll
+      for (int d = 1; d < WAVE; d <<= 1) {
+        const unsigned x = __shfl_up(scan, d, WAVE);
+        if (lane >= d) scan += x;
+      }
+      if (lane == WAVE - 1) wave_totals[wid] = scan;
+    }
+    __syncthreads();
+    if (tid < DIGITS) {
+      unsigned run = scan - total;
+      for (int w = 0; w < wid; ++w) run += wave_totals[w];
+#pragma unroll
+      for (int w = 0; w < ONE_WAVES; ++w) {
+        const unsigned c = offs[w][tid];
+        offs[w][tid] = run;
+        run += c;
+      }
+    }
+    __syncthreads();
+    volatile unsigned* mine = offs[wid];
+#pragma unroll
+    for (int j = 0; j < ONE_ITEMS; ++j) {
+      const bool live = i0 + j * WAVE < N;
+      const unsigned digit = (key[j] >> shift) & 255u;
+      unsigned long long same = __ballot(live);
+#pragma unroll
+      for (int bit = 0; bit < 8; ++bit) {
+        const unsigned long long one = __ballot((digit >> bit) & 1u);
+        same &= ((digit >> bit) & 1u) ? one : ~one;
+      }
+      if (live) {
+        const int rank = __popcll(same & ((1ull << lane) - 1ull));
+        const unsigned at = mine[digit];
+        __builtin_amdgcn_wave_barrier();
+        if (rank == 0) mine[digit] = at + (unsigned)__popcll(same);
+        s_key[at + rank] = key[j];
+        s_pos[at + rank] = pos[j];
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ONE_ITEMS; ++j) {
+      const int i = i0 + j * WAVE;
+      if (i < N) {
+        key[j] = s_key[i];
+        pos[j] = s_pos[i];
+      }
+    }
+    // (the next pass's two barriers stand between these reads and its writes)
+  }
+#pragma unroll
+  for (int j = 0; j < ONE_ITEMS; ++j) {
+    const int i = i0 + j * WAVE;
+    if (i < N) {
+      keys_out[i] = key[j];
+      pos_out[i] = pos[j];
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Backward, step 2: sums over CHUNK sorted positions, COLS columns a wave.
 // A segment (one token's positions) inside its chunk is final; one that came
@@ -486,53 +597,65 @@ torch::Tensor embedding_bwd(const torch::Tensor& dy_in,
   const int rounds =
       (int)((N + (long)SORT_TILE * SORT_BLOCKS - 1) / ((long)SORT_TILE * SORT_BLOCKS));
   const long tile = (long)rounds * SORT_TILE;
-  const int nblk = (int)((N + tile - 1) / tile);
+  const bool one_block = N <= ONE_BLOCK_IDS;
+  const int nblk = one_block ? 1 : (int)((N + tile - 1) / tile);
   const long chunks = (N + CHUNK - 1) / CHUNK;
 
-  auto iopt = dy.options().dtype(at::kInt);
-  auto sorted = torch::empty({4, N}, iopt);  // two pairs of (key, position)
-  auto counts = torch::empty({(long)nblk * DIGITS}, iopt);
-  auto parts = torch::empty({2, chunks, (long)D}, dy.options().dtype(at::kFloat));
-  unsigned* sp = (unsigned*)sorted.data_ptr();
-  unsigned* cp = (unsigned*)counts.data_ptr();
+  // One workspace: heads and tails, the sorted (key, position) pairs twice,
+  // the counts.
+  const long parts = 2 * chunks * D, sorted = one_block ? 2 * N : 4 * N;
+  auto space = torch::empty({parts + sorted + (long)nblk * DIGITS},
+                            dy.options().dtype(at::kFloat));
+  float* head = space.data_ptr<float>();
+  float* tail = head + chunks * D;
+  unsigned* sp = (unsigned*)(head + parts);
+  unsigned* cp = sp + sorted;
   const auto stream = cur_stream();
-  int at_pair = 0;
   // The gradient's 16-byte words in shares: one for each counting kernel, two
   // for each (longer) scatter kernel. Its last bytes are cleared by themselves.
   const long bytes = dw.numel() * (long)dw.element_size();
   const long words = bytes / 16;
   if (bytes % 16 != 0)
     dw.flatten().slice(0, words * 16 / (long)dw.element_size()).zero_();
-  const int shares = 3 * passes;
+  const int shares = one_block ? 1 : 3 * passes;
   auto share = [&](int from, int to) {
     const long a = words * from / shares, b = words * to / shares;
     return Fill{(uint4*)dw.data_ptr() + a, b - a, nblk};
   };
-  auto blocks = [&](const Fill& f) {  // four stores a thread, 4096 blocks at most
-    return dim3(nblk + (unsigned)std::min<long>((f.n + 1023) / 1024, 4096));
+  // four stores a thread, 4096 blocks of 256 at most
+  auto blocks = [&](const Fill& f, int threads) {
+    return dim3(nblk + (unsigned)std::min<long>((f.n + 4 * threads - 1) / (4 * threads),
+                                                4096 * EMB_BLOCK / threads));
   };
+  int at_pair = 0;
   DISPATCH_IDS(ids, {
     const id_t* ip = (const id_t*)ids.data_ptr();
-    for (int p = 0; p < passes; ++p) {
+    if (one_block) {
+      const Fill f = share(0, 1);
+      auto sort = N <= 4 * ONE_BLOCK ? sort_one_block_kernel<id_t, 4>
+                                     : sort_one_block_kernel<id_t, 16>;
+      hipLaunchKernelGGL(sort, blocks(f, ONE_BLOCK), dim3(ONE_BLOCK), 0, stream,
+                         ip, sp, sp + N, (int)N, V, passes, f);
+      at_pair = 1;
+    }
+    for (int p = 0; !one_block && p < passes; ++p) {
       unsigned* in = sp + (long)(1 - at_pair) * 2 * N;
       unsigned* to = sp + (long)at_pair * 2 * N;
       const Fill f0 = share(3 * p, 3 * p + 1), f1 = share(3 * p + 1, 3 * p + 3);
       auto count = p == 0 ? sort_count_kernel<id_t, true>
                           : sort_count_kernel<id_t, false>;
-      hipLaunchKernelGGL(count, blocks(f0), dim3(EMB_BLOCK), 0, stream, ip, in,
-                         (int)N, V, rounds, 8 * p, cp, f0);
+      hipLaunchKernelGGL(count, blocks(f0, EMB_BLOCK), dim3(EMB_BLOCK), 0,
+                         stream, ip, in, (int)N, V, rounds, 8 * p, cp, f0);
       auto scatter = p == 0 ? sort_scatter_kernel<id_t, true>
                             : sort_scatter_kernel<id_t, false>;
-      hipLaunchKernelGGL(scatter, blocks(f1), dim3(EMB_BLOCK), 0, stream, ip,
-                         in, in + N, to, to + N, (int)N, V, rounds, 8 * p, cp,
-                         f1);
+      hipLaunchKernelGGL(scatter, blocks(f1, EMB_BLOCK), dim3(EMB_BLOCK), 0,
+                         stream, ip, in, in + N, to, to + N, (int)N, V, rounds,
+                         8 * p, cp, f1);
       at_pair = 1 - at_pair;
     }
   });
   const unsigned* keys = sp + (long)(1 - at_pair) * 2 * N;
   const unsigned* pos = keys + N;
-  float* head = parts.data_ptr<float>();
-  float* tail = head + chunks * D;
   const bool wide = D % 4 == 0 && aligned(dy.data_ptr(), 4 * (int)dy.element_size());
   const bool wider = wide && dy.element_size() == 2 && D % 8 == 0 &&
                      aligned(dy.data_ptr(), 16);

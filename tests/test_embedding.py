@@ -124,6 +124,16 @@ def test_many_ids_over_all_sort_blocks(dev):
 
 
 @gpu
+@pytest.mark.parametrize("n", [4096, 4097, 16383, 16384, 16385])
+@pytest.mark.parametrize("V", [200, 300, 70000, 20_000_000])
+def test_both_sorts_over_one_to_four_passes(dev, n, V):
+    """Either side of the longest lists that one workgroup sorts."""
+    w, ids, dy = make(dev, n, V, 4, BF16, F32, skew=V < 70000)
+    (g,) = torch.autograd.grad(embedding(ids, w, 1.0, F32), w, dy)
+    assert_grad(g, ids, dy, 1.0)
+
+
+@gpu
 @pytest.mark.parametrize("n", [1, 32, 33, 64, 3000])
 def test_one_token_everywhere(dev, n):
     w, ids, dy = make(dev, n, 1000, 768, F32, BF16)
