@@ -69,6 +69,7 @@ def run_icl_eval(cfg, model, device) -> dict:
         return {}
     from .data.convert import load_tokenizer
     from .eval import evaluate_icl_tasks, gauntlet_composite
+    from .models import MPTCausalLM
 
     tok = load_tokenizer(icl_cfg.get("tokenizer_path"))
     # fp32 weights on a GPU: the flash kernels take bf16
@@ -79,7 +80,9 @@ def run_icl_eval(cfg, model, device) -> dict:
             model, tasks, tok, device=device,
             max_seq_len=int(cfg["llm_config"].get("max_seq_len", 2048)),
             limit_examples=icl_cfg.get("limit_examples"),
-            share_prefix=bool(icl_cfg.get("share_prefix", False)),
+            # not with a wrapper that gathers parameters in its own forward
+            share_prefix=bool(icl_cfg.get("share_prefix", False))
+            and isinstance(model, MPTCausalLM),
         )
     gauntlet = (cfg.get("eval_gauntlet_config") or {}).get("eval_gauntlet")
     results.update(gauntlet_composite(results, gauntlet))

@@ -285,8 +285,12 @@ std::vector<torch::Tensor> clip_grads(std::vector<torch::Tensor> gs,
     hipLaunchKernelGGL(clip_kernel, dim3(plan.grids[i]), dim3(GN_BLOCK), 0,
                        cur_stream(), plan.lists[i],
                        result[0].data_ptr<float>(), (float)max_norm);
-  for (size_t i = 0; i < gs.size(); ++i)
-    if (plan.copied[i]) gs[i].copy_(plan.t[i]);
+  for (size_t i = 0; i < gs.size(); ++i) {
+    if (plan.copied[i])
+      gs[i].copy_(plan.t[i]);
+    else
+      gs[i].unsafeGetTensorImpl()->bump_version();  // written in place
+  }
   return result;
 }
 

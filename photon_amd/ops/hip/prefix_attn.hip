@@ -219,6 +219,7 @@ torch::Tensor prefix_attention_decode(torch::Tensor qkv, torch::Tensor prefix,
                      a.info.data_ptr<int>(), part.o, part.ml,
                      (__bf16*)out.data_ptr(), a.H, (int)cache.size(1), c.rows,
                      c.items, c.splits);
+  cache.unsafeGetTensorImpl()->bump_version();  // written in place
   return out;
 }
 

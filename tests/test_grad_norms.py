@@ -153,6 +153,16 @@ def test_pieces_that_begin_anywhere(dev):
 
 
 @gpu
+def test_in_place_writes_are_known_to_autograd(dev):
+    """A gradient that a later backward still needs is refused after it."""
+    x = torch.randn(50, device=dev, requires_grad=True)
+    y = x.exp()  # its result is saved for the backward
+    clip_grads_([y.detach()], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+
+
+@gpu
 def test_strided_gradients(dev):
     a = torch.randn(64, 48, device=dev)
     b = torch.randn(33, 40, device=dev).to(BF16)

@@ -146,6 +146,29 @@ def test_icl_tasks_score_the_same(tmp_path):
     assert a == b and len(a) == 12
 
 
+def test_eval_path_of_centralised_training(tmp_path):
+    """run_icl_eval reads icl_tasks_config.share_prefix; a wrapped model runs
+    option by option."""
+    from photon_amd.centralised_train import run_icl_eval
+
+    tasks = write_tasks(tmp_path)
+    got = {}
+    for share in (False, True):
+        cfg = {"icl_tasks_config": {"icl_tasks": tasks, "share_prefix": share}, "llm_config": {"max_seq_len": 128}}
+        got[share] = run_icl_eval(cfg, tiny(vocab=512), "cpu")
+    assert got[False] == got[True] and len(got[True]) >= 12
+
+    class Wrapped(torch.nn.Module):
+        def __init__(self, inner):
+            super().__init__()
+            self.inner = inner
+
+        def forward(self, *a, **k):
+            return self.inner(*a, **k)
+
+    assert run_icl_eval(cfg, Wrapped(tiny(vocab=512)), "cpu") == got[False]
+
+
 def test_emb_scale_in_the_model():
     """emb_scale is read from the configuration, survives a resize, and 1.0
     leaves the model as it was."""
