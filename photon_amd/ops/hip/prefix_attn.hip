@@ -30,8 +30,12 @@ using ManyRows = Shape<D, 4, 1, 2>;
 constexpr long FEW_ITEMS = 128;
 
 // Whole rounds of items fill the chip by themselves; what is left over is
-// split until it does, but not below two key tiles (one a wave with few rows)
-// each. `always`: every item leaves partial rows.
+// split until it does, but not below some keys each. With many rows these are
+// two tiles. With few rows a split call is bound by the host's two launches,
+// 10 us: 20 rows of 12 heads of 64 over 701 keys take 8.7 us whole and 10.0 in
+// two, 96 rows of 16 heads of 128 over 1507 keys 20.7 whole and 15.4 in four.
+// `always` (the decode form, which joins anyway): every item leaves partial
+// rows; one sequence over 701 keys takes 12.0 us whole and 10.7 in two.
 Cut cut(long T, int H, int D, long keys, bool always) {
   Cut c;
   c.few = (T + FewRows<64>::ROWS - 1) / FewRows<64>::ROWS * H <= FEW_ITEMS;
@@ -45,7 +49,9 @@ Cut cut(long T, int H, int D, long keys, bool always) {
   c.rest = c.items - c.full;
   c.splits = 1;
   if (c.rest > 0 && c.rest < at_once)
-    c.splits = (int)std::max(1L, std::min<long>(at_once / c.rest, keys / 128));
+    c.splits = (int)std::max(
+        1L, std::min<long>(at_once / c.rest,
+                           keys / (!c.few ? 128 : always ? 256 : 384)));
   if (c.splits == 1 && !always) {
     c.full = c.items;
     c.rest = 0;
