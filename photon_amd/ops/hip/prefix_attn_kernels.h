@@ -15,8 +15,18 @@
 // The key axis can be split over workgroups: each leaves (m, l, o) with
 // m = max w, l = sum e^(w - m), o = sum e^(w - m) v, and
 //   M = max m_i,  o = sum e^(m_i - M) o_i / sum e^(m_i - M) l_i
-// joins them. Statistics and sums are fp32; the probabilities are rounded to
-// bf16 for the second matrix product, as the values they weigh are.
+// joins them. Statistics and sums are fp32; the weights are rounded to bf16 for
+// the second matrix product, as the values they weigh are (2^-8 of each weight
+// at most, and the result's own rounding is as large).
+//
+// Measured on an MI355X. Many rows (4416 over 3901 shared keys, 32 heads of
+// 128): 294 us for 290 GFLOP, of which 237 are computed (far keys of steep heads
+// are not weighed). Of the SIMDs' cycles products take 34%, vector instructions
+// 32%, LDS accesses 21% of the CUs'; of two waves a SIMD 1.5 are there on average.
+// Few rows (93 over 1507, 16 heads of 128): 12 us and 4 for the join, a chain of
+// latencies. One new token for each of 64 sequences over 3967 keys and caches of
+// 512, 32 heads of 128: 20 us for the prefix (66 MB) and 60 for the caches
+// (267 MB, 4.4 TB/s).
 
 #pragma once
 
@@ -158,13 +168,13 @@ __global__ __launch_bounds__(S::THREADS, S::D == 64 ? 3 : 2) void prefix_attn_ke
   // own position of this lane's row, and the first packed row it may see
   int first = 0, own = 0;
   if (DECODE) {
-    own = max(info[row], 0);
+    own = min(max(info[row], 0), 1 << 30);
   } else {
     first = min(max(info[row], 0), row);
     own = row - first;
   }
 
-  // key tiles: the prefix's, then the packed rows lo..hi_row of this block
+  // key tiles: the prefix's, then the packed rows lo .. end_row - 1
   const int n_pre = (P + KEYS - 1) / KEYS;
   int lo = 0, n_own = 0, end_row = 0;
   if (!DECODE) {
@@ -427,7 +437,8 @@ __global__ __launch_bounds__(S::THREADS, S::D == 64 ? 3 : 2) void prefix_attn_ke
         __builtin_elementwise_maximum(top[0], top[SUBS - 1]));
     // Below 2^-150 of the maximum a weight is zero in fp32: a tile of such
     // weights (far keys of a steep head, other sequences' rows) adds nothing.
-    // A NaN among the scores makes the comparison false.
+    // A NaN among the scores makes the comparison false; one among a prefix
+    // tile's values is not looked for under weights that are all zero.
     if (!bad && __all(highest - m_run < -150.f)) continue;
     raise(highest);
 #pragma unroll

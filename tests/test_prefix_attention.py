@@ -179,6 +179,10 @@ def test_packed_rows(dev, D, P, lens):
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("lens,P,H", [
     ([1] * 130, 333, 1), ([7, 100] * 20, 129, 12), ([1500], 63, 2), ([300, 700, 20], 0, 2), ([3] * 4, 4000, 1),
+    # more than 128 items of 32 rows: tiles of 128 rows
+    ([300, 700, 20], 0, 12), ([1] * 1000, 65, 12), ([500, 1, 0, 40], 1, 20), ([2, 3], 700, 150), ([4099], 31, 2),
+    # whole rounds of workgroups, and a rest that is split
+    ([90] * 50, 520, 16),
 ])
 def test_packed_rows_larger(dev, D, lens, P, H):
     check(dev, lens, P, H, D)
@@ -191,8 +195,9 @@ def test_no_rows(dev):
 
 
 @gpu
-def test_strides_and_alignment(dev):
-    H, D, lens, P = 2, 64, [5, 60, 9], 100
+@pytest.mark.parametrize("H", [2, 48])
+def test_strides_and_alignment(dev, H):
+    D, lens, P = 64, [5, 60, 9], 100
     qkv, prefix, slopes = make(dev, 74, P, H, D)
     starts = sequence_starts(lens, dev)
     want = prefix_attention_qkv(qkv, prefix, H, slopes, starts)
@@ -212,10 +217,11 @@ def test_strides_and_alignment(dev):
 
 
 @gpu
-def test_sequences_do_not_touch_each_other(dev):
+@pytest.mark.parametrize("H,D", [(2, 64), (48, 64), (2, 128), (48, 128)])
+def test_sequences_do_not_touch_each_other(dev, H, D):
     """Infinities and NaN of one sequence stay in it, and a later row's stay
     out of the earlier rows of its sequence."""
-    H, D, lens, P = 2, 64, [5, 60, 9, 1], 100
+    lens, P = [5, 60, 9, 1], 100
     qkv, prefix, slopes = make(dev, 75, P, H, D)
     starts = sequence_starts(lens, dev)
     out, mag = exact(qkv, prefix, H, slopes, lens)
@@ -238,9 +244,28 @@ def test_sequences_do_not_touch_each_other(dev):
 
 
 @gpu
-def test_starts_out_of_range_stay_inside(dev):
+def test_not_finite_in_the_prefix(dev):
+    """What every row sees reaches every row."""
+    H, D, lens, P = 1, 64, [3, 40], 200
+    qkv, prefix, slopes = make(dev, 43, P, H, D)
+    starts = sequence_starts(lens, dev)
+    for row, part, bad in ((199, 1, float("nan")), (0, 1, float("nan")), (199, 2, float("nan")), (199, 2, float("inf"))):
+        x = prefix.clone()
+        x[row, part * D + 5] = bad
+        got = prefix_attention_qkv(qkv, x, H, slopes * 1e-3, starts)
+        if part == 1:
+            assert got.isnan().all()
+        else:
+            assert bool((got[:, 5].isnan() if math.isnan(bad) else got[:, 5] == bad).all())
+            rest = torch.arange(D, device=dev) != 5
+            assert got[:, rest].isfinite().all()
+
+
+@gpu
+@pytest.mark.parametrize("H", [1, 70])
+def test_starts_out_of_range_stay_inside(dev, H):
     """Starts that no packing gives are read as the nearest that one could."""
-    H, D, P = 1, 64, 70
+    D, P = 64, 70
     qkv, prefix, slopes = make(dev, 40, P, H, D)
     starts = torch.full((40,), -5, dtype=torch.int32, device=dev)
     starts[20:] = 1000
@@ -251,10 +276,13 @@ def test_starts_out_of_range_stay_inside(dev):
 
 @gpu
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("B,P,slots", [(1, 0, 1), (1, 701, 24), (3, 64, 7), (33, 65, 40), (70, 300, 130), (2, 5, 700)])
-def test_decode(dev, D, B, P, slots):
+@pytest.mark.parametrize("B,P,slots,H", [
+    (1, 0, 1, 3), (1, 701, 24, 3), (3, 64, 7, 3), (33, 65, 40, 3), (70, 300, 130, 3), (2, 5, 700, 3),
+    (1, 3000, 5, 1),  # more splits than are asked for early
+    (400, 130, 9, 12), (130, 1, 3, 40),  # more than 128 items of 32 rows
+])
+def test_decode(dev, D, B, P, slots, H):
     """Against the packed form's definition, with NaN in every unused slot."""
-    H = 3
     held = [(17 * i + slots - 1) % slots for i in range(B)]
     lens = [n + 1 for n in held]
     qkv, prefix, slopes = make(dev, sum(lens), P, H, D)
