@@ -178,7 +178,7 @@ torch::Tensor prefix_attention(torch::Tensor qkv, torch::Tensor prefix, long H,
     hipLaunchKernelGGL(join, dim3((unsigned)((threads + 255) / 256)),
                        dim3(256), 0, cur_stream(), part.o, part.ml,
                        (__bf16*)out.data_ptr(), a.T, a.H, c.rows, c.full,
-                       c.rest, c.splits);
+                       c.rest, c.splits, !c.few && a.H % 8 == 0);
   }
   return out;
 }

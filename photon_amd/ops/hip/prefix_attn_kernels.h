@@ -124,6 +124,24 @@ DEV_INLINE bf16x8 pack_weights(const float* p) {
   return out.v;
 }
 
+// Which query tile and head an item is. `by_head` (many rows, a multiple of 8
+// heads): workgroup i runs on XCD i % 8, so each XCD takes one of every 8 heads,
+// in turn from below and from above, and its tiles one head after the other, the
+// flattest first: where slopes fall with the head's number, as ALiBi's do, what
+// comes last is short. Otherwise tile by tile.
+DEV_INLINE void place(int item, int H, int tiles, bool by_head, int& tile,
+                      int& h) {
+  if (by_head) {
+    const int x = item & 7, j = item >> 3;
+    const int g = H / 8 - 1 - j / tiles;
+    tile = j % tiles;
+    h = 8 * g + (g & 1 ? 7 - x : x);
+  } else {
+    tile = item / H;
+    h = item % H;
+  }
+}
+
 // Swapped product (keys x queries): lane holds query lane & 31, its 16
 // registers the keys (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5) of 32.
 //
@@ -154,8 +172,10 @@ __global__ __launch_bounds__(S::THREADS, S::D == 64 ? 3 : 2) void prefix_attn_ke
     item = full + (item - full) / splits;
     parts = splits;
   }
-  const int h = item % H;
-  const int q0_block = item / H * (NW * QB);
+  int tile, h;
+  place(item, H, (T + S::ROWS - 1) / S::ROWS, !DECODE && KW == 1 && H % 8 == 0,
+        tile, h);
+  const int q0_block = tile * S::ROWS;
   const int my_q = q0_block + rw * QB + lq;
   const int row = min(my_q, T - 1);
 
@@ -549,14 +569,15 @@ template <int D>
 __global__ __launch_bounds__(256) void prefix_join_kernel(
     const float* __restrict__ part_o, const float* __restrict__ part_ml,
     __bf16* __restrict__ out, int T, int H, int rows, int full, int rest,
-    int splits) {
+    int splits, bool by_head) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   const long pr = i / (D / 4);  // partial row: [item - full][row]
   const int col = (int)(i % (D / 4)) * 4;
   if (pr >= (long)rest * rows) return;
   const int item = full + (int)(pr / rows);
-  const int h = item % H;
-  const long t = (long)(item / H) * rows + pr % rows;
+  int tile, h;
+  place(item, H, (T + rows - 1) / rows, by_head, tile, h);
+  const long t = (long)tile * rows + pr % rows;
   if (t >= T) return;
   const long stride = (long)rest * rows;
   float M = -1e30f;
