@@ -11,11 +11,11 @@ namespace photon_hip {
 namespace {
 
 // How a call is cut into workgroups: items of `rows` query rows of one head,
-// the last `rest` of them split `splits` times along the keys.
+// `rest` of them, from `first_split` on, split `splits` times along the keys.
 struct Cut {
   bool few;  // few rows: waves share the keys, not the rows
-  int rows, items, full, rest, splits;
-  int groups() const { return full + rest * splits; }
+  int rows, items, first_split, rest, splits;
+  int groups() const { return items + rest * (splits - 1); }
   long partial_rows() const { return (long)rest * splits * rows; }
 };
 
@@ -30,7 +30,10 @@ using ManyRows = Shape<D, 4, 1, 2>;
 constexpr long FEW_ITEMS = 128;
 
 // Whole rounds of items fill the chip by themselves; what is left over is
-// split until it does, but not below some keys each. With many rows these are
+// split until it does, but not below some keys each. The split ones come right
+// after the first round, where heads that see the whole prefix are still on:
+// the short ones that follow fill the gaps (4416 rows over 3901 keys, 32 heads of
+// 128: 261 us with the split ones last, 232 so). With many rows these are
 // two tiles. With few rows a split call is bound by the host's two launches,
 // 10 us: 20 rows of 12 heads of 64 over 701 keys take 8.7 us whole and 10.0 in
 // two, 96 rows of 16 heads of 128 over 1507 keys 20.7 whole and 15.4 in four.
@@ -45,32 +48,30 @@ Cut cut(long T, int H, int D, long keys, bool always) {
   c.items = (int)items;
   // workgroups that are on the chip together, by their registers and LDS
   const int at_once = c.few ? (D == 64 ? 512 : 256) : (D == 64 ? 768 : 512);
-  c.full = always ? 0 : c.items / at_once * at_once;
-  c.rest = c.items - c.full;
+  c.rest = always ? c.items : c.items % at_once;
+  c.first_split = c.items > c.rest ? at_once : 0;
   c.splits = 1;
   if (c.rest > 0 && c.rest < at_once)
     c.splits = (int)std::max(
         1L, std::min<long>(at_once / c.rest,
                            keys / (!c.few ? 128 : always ? 256 : 384)));
-  if (c.splits == 1 && !always) {
-    c.full = c.items;
-    c.rest = 0;
-  }
+  if (c.splits == 1 && !always) c.rest = 0;
   return c;
 }
 
 template <bool DECODE>
 void launch(const torch::Tensor& qkv, const torch::Tensor& prefix, int H,
             int D, const torch::Tensor& slopes, const torch::Tensor& info,
-            __bf16* out, float* part_o, float* part_ml, int T, int P,
+            const float* norms, __bf16* out, float* part_o, float* part_ml, int T, int P,
             const Cut& c) {
   const __bf16* pre = (const __bf16*)prefix.data_ptr();
   const __bf16* pk = pre + (long)H * D;
   const __bf16* pv = pre + 2L * H * D;
 #define ARGS                                                                 \
   cur_stream(), (const __bf16*)qkv.data_ptr(), qkv.stride(0), pk, pv,        \
-      prefix.stride(0), slopes.data_ptr<float>(), info.data_ptr<int>(), out, \
-      part_o, part_ml, T, P, H, c.full, c.splits
+      prefix.stride(0), slopes.data_ptr<float>(), info.data_ptr<int>(),      \
+      norms, out, part_o, part_ml, T, P, H, c.first_split, c.rest,                  \
+      c.splits
 #define LAUNCH(SHAPE)                                                        \
   hipLaunchKernelGGL((prefix_attn_kernel<SHAPE, DECODE>), dim3(c.groups()),  \
                      dim3(SHAPE::THREADS), SHAPE::BYTES, ARGS)
@@ -170,14 +171,29 @@ torch::Tensor prefix_attention(torch::Tensor qkv, torch::Tensor prefix, long H,
   if (a.T == 0) return out;
   const Cut c = cut(a.T, a.H, a.D, (long)a.P + 64, false);
   const Partial part(c, a.D, qkv);
+  torch::Tensor norms;
+  // The keys' lengths, by which far tiles are left out, where that is worth the
+  // pass: more than one round of workgroups (in one, the flattest head's take as
+  // long as before) over a long prefix. 32 heads of 128, 4000 rows: 237 us
+  // without and 195 with over 4000 keys, 145 and 143 over 2000, 93 and 94 over
+  // 1000; 2000 rows (one round) over 4000 keys 121 and 120.
+  if (c.first_split > 0 && a.P >= 2500) {
+    const int tiles = (a.P + NORM_KEYS - 1) / NORM_KEYS;
+    norms = torch::empty({(long)a.H * tiles}, qkv.options().dtype(at::kFloat));
+    auto fn = a.D == 64 ? key_norms_kernel<64> : key_norms_kernel<128>;
+    hipLaunchKernelGGL(fn, dim3(a.H, tiles), dim3(256), 0, cur_stream(),
+                       (const __bf16*)a.prefix.data_ptr() + (long)a.H * a.D,
+                       a.prefix.stride(0), norms.data_ptr<float>(), a.P);
+  }
   launch<false>(a.qkv, a.prefix, a.H, a.D, a.slopes, a.info,
+                norms.defined() ? norms.data_ptr<float>() : nullptr,
                 (__bf16*)out.data_ptr(), part.o, part.ml, a.T, a.P, c);
   if (c.rest) {
     const long threads = (long)c.rest * c.rows * a.D / 4;
     auto join = a.D == 64 ? prefix_join_kernel<64> : prefix_join_kernel<128>;
     hipLaunchKernelGGL(join, dim3((unsigned)((threads + 255) / 256)),
                        dim3(256), 0, cur_stream(), part.o, part.ml,
-                       (__bf16*)out.data_ptr(), a.T, a.H, c.rows, c.full,
+                       (__bf16*)out.data_ptr(), a.T, a.H, c.rows, c.first_split,
                        c.rest, c.splits, !c.few && a.H % 8 == 0);
   }
   return out;
@@ -214,7 +230,8 @@ torch::Tensor prefix_attention_decode(torch::Tensor qkv, torch::Tensor prefix,
   if (a.P > 0) c = cut(B, a.H, a.D, a.P, true);
   const Partial part(c, a.D, qkv);
   if (a.P > 0)
-    launch<true>(a.qkv, a.prefix, a.H, a.D, a.slopes, a.info, nullptr, part.o,
+    launch<true>(a.qkv, a.prefix, a.H, a.D, a.slopes, a.info, nullptr,
+                 nullptr, part.o,
                  part.ml, a.T, a.P, c);
   auto own = a.D == 64 ? decode_own_kernel<64> : decode_own_kernel<128>;
   hipLaunchKernelGGL(own, dim3(a.H, (unsigned)B), dim3(OWN_BLOCK), 0,

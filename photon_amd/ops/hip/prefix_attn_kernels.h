@@ -19,14 +19,19 @@
 // the second matrix product, as the values they weigh are (2^-8 of each weight
 // at most, and the result's own rounding is as large).
 //
+// Below 2^-150 of a row's maximum a weight is zero in fp32, and ALiBi makes most
+// far keys of a steep head that: their tiles are left out after the first product
+// (the scores say so) or, with many rows over a long prefix, before they are
+// loaded (Cauchy and Schwarz: q . k <= |q| max |k|, see key_norms_kernel).
+//
 // Measured on an MI355X. Many rows (4416 over 3901 shared keys, 32 heads of
-// 128): 294 us for 290 GFLOP, of which 237 are computed (far keys of steep heads
-// are not weighed). Of the SIMDs' cycles products take 34%, vector instructions
-// 32%, LDS accesses 21% of the CUs'; of two waves a SIMD 1.5 are there on average.
-// Few rows (93 over 1507, 16 heads of 128): 12 us and 4 for the join, a chain of
-// latencies. One new token for each of 64 sequences over 3967 keys and caches of
-// 512, 32 heads of 128: 20 us for the prefix (66 MB) and 60 for the caches
-// (267 MB, 4.4 TB/s).
+// 128): 232 us, of which 8 go to the keys' lengths and 8 to the join; 290 GFLOP
+// by the formula, 174 computed. Of the SIMDs' cycles matrix instructions take
+// 32% and vector instructions 38% with little overlap, LDS accesses 22% of the
+// CUs'; the rest is waiting, at 1.6 waves a SIMD of 2. Few rows (93 over 1507, 16
+// heads of 128): 12 us and 4 for the join, a chain of latencies. One new token
+// for each of 64 sequences over 3967 keys and caches of 512, 32 heads of 128: 20
+// us for the prefix (66 MB) and 60 for the caches (267 MB, 4.4 TB/s).
 
 #pragma once
 
@@ -124,11 +129,53 @@ DEV_INLINE bf16x8 pack_weights(const float* p) {
   return out.v;
 }
 
+// The largest |k|^2 of each head and NORM_KEYS keys of the prefix, [H][tiles];
+// NaN if one of them is. A workgroup reads these keys of one head, D / 8 lanes
+// each. Bound by memory: 32 MB (3901 keys, 32 heads of 128) in 8 us.
+constexpr int NORM_KEYS = 64;
+DEV_INLINE int norm_tiles(int P) { return (P + NORM_KEYS - 1) / NORM_KEYS; }
+template <int D>
+__global__ __launch_bounds__(256) void key_norms_kernel(
+    const __bf16* __restrict__ pk, long p_rs, float* __restrict__ norms,
+    int P) {
+  constexpr int L = D / 8, G = 256 / L;
+  __shared__ float s_max[4];
+  const int h = blockIdx.x, tile = blockIdx.y;
+  const int g = threadIdx.x / L, c = threadIdx.x % L * 8;
+  const __bf16* at = pk + (long)h * D + c;
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < NORM_KEYS / G; ++i) {
+    const int key = tile * NORM_KEYS + i * G + g;
+    float sum = 0.f;
+    if (key < P) {
+      const bf16x8 x = *(const bf16x8*)(at + (long)key * p_rs);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum = fmaf((float)x[j], (float)x[j], sum);
+    }
+#pragma unroll
+    for (int off = L / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off, WAVE);
+    top = __builtin_elementwise_maximum(top, sum);  // NaN stays
+  }
+#pragma unroll
+  for (int off = 32; off >= L; off >>= 1)
+    top = __builtin_elementwise_maximum(top, __shfl_xor(top, off, WAVE));
+  if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < 4; ++w)
+      top = __builtin_elementwise_maximum(top, s_max[w]);
+    norms[(long)h * gridDim.y + tile] = top;
+  }
+}
+
 // Which query tile and head an item is. `by_head` (many rows, a multiple of 8
 // heads): workgroup i runs on XCD i % 8, so each XCD takes one of every 8 heads,
 // in turn from below and from above, and its tiles one head after the other, the
 // flattest first: where slopes fall with the head's number, as ALiBi's do, what
-// comes last is short. Otherwise tile by tile.
+// comes last is short (294 -> 275 us at the many rows above). Otherwise tile by
+// tile.
 DEV_INLINE void place(int item, int H, int tiles, bool by_head, int& tile,
                       int& h) {
   if (by_head) {
@@ -153,23 +200,28 @@ __global__ __launch_bounds__(S::THREADS, S::D == 64 ? 3 : 2) void prefix_attn_ke
     const __bf16* __restrict__ qkv, long q_rs, const __bf16* __restrict__ pk,
     const __bf16* __restrict__ pv, long p_rs,
     const float* __restrict__ slopes, const int* __restrict__ info,
-    __bf16* __restrict__ out, float* __restrict__ part_o,
-    float* __restrict__ part_ml, int T, int P, int H, int full, int splits) {
+    const float* __restrict__ norms, __bf16* __restrict__ out,
+    float* __restrict__ part_o, float* __restrict__ part_ml, int T, int P,
+    int H, int first_split, int rest, int splits) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int D = S::D, NW = S::NW, KW = S::KW, BUFS = S::BUFS;
   constexpr int SUBS = S::SUBS, KEYS = S::KEYS, IMG = S::IMG;
   constexpr bool D64 = D == 64;
+  constexpr bool STOPS = KW == 1 && BUFS == 2 && !DECODE;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rw = wave % NW, kw = wave / NW;  // rows, keys of this wave
   const int hi = lane >> 5;
   const int lq = lane & 31;
-  // the first `full` items (query tile, head) are whole, the others split
+  // `rest` items from `first_split` on are split, the others whole
   int item = blockIdx.x, split = 0, parts = 1;
-  if (item >= full) {
-    split = (item - full) % splits;
-    item = full + (item - full) / splits;
+  if (item >= first_split + rest * splits) {
+    item -= rest * (splits - 1);
+  } else if (item >= first_split) {
+    const int i = item - first_split;
+    split = KW == 1 ? i / rest : i % splits;  // many rows: on its head's XCD
+    item = first_split + (KW == 1 ? i % rest : i / splits);
     parts = splits;
   }
   int tile, h;
@@ -268,6 +320,35 @@ __global__ __launch_bounds__(S::THREADS, S::D == 64 ? 3 : 2) void prefix_attn_ke
   f32x16 o_acc[D / 32];
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) o_acc[db] = f32x16{};
+
+  // What no score with a key of the prefix exceeds: |q| times the longest key
+  // (the factor is for the rounding of both). The row's score with its own key
+  // is a bound from below of its maximum, also where the keys are split.
+  float bound = INFINITY;
+  if (STOPS && norms != nullptr) {
+    float longest = 0.f, qq = 0.f, self = 0.f;
+    for (int i = lane; i < norm_tiles(P); i += 64)
+      longest = __builtin_elementwise_maximum(longest,
+                                              norms[(long)h * norm_tiles(P) + i]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1)
+      longest = __builtin_elementwise_maximum(
+          longest, __shfl_xor(longest, off, WAVE));
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const bf16x8 own_k = *(const bf16x8*)(k + row * q_rs + kk * 16 + 8 * hi);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = (float)qfrag[kk][j];
+        qq = fmaf(x, x, qq);
+        self = fmaf(x, (float)own_k[j], self);
+      }
+    }
+    qq += __shfl_xor(qq, 32, WAVE);
+    self += __shfl_xor(self, 32, WAVE);
+    bound = sqrtf(qq * longest) * scale2 * 1.001f;
+    m_run = fmaxf(m_run, self * scale2);
+  }
 
   // The accumulators of the scores begin at slope * sqrt(d) * (key within the
   // subtile); the rest of the bias is a constant of row and subtile that joins
@@ -420,10 +501,24 @@ __global__ __launch_bounds__(S::THREADS, S::D == 64 ? 3 : 2) void prefix_attn_ke
     else
       vm_wait0();
     // tile t is there, and the reads of the one before are done
+    const bool look = STOPS && norms != nullptr && (t & 3) == 0 && t < n_pre;
+    int* const done = bad_words + NW;  // read long before the next is written
+    if (look) {
+      // ALiBi takes this much, or more, from the tiles up to t
+      const float most = bound + slope2 * (float)((t + 1) * KEYS - 1 - P - own);
+      const bool all = __all(most - m_run < -150.f) && slope2 >= 0.f;
+      if (lane == 0) done[rw] = all;
+    }
     if (KW == 1)
       __syncthreads();
     else
       lds_wait0();
+    if (look) {
+      bool all = true;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) all &= done[w] != 0;
+      if (all) break;  // nothing is on its way
+    }
     if (t - (BUFS - 1) * KW >= t0) stage(t - (BUFS - 1) * KW, old);
     const bool pre = t < n_pre;
     const int kv0 = pre ? t * KEYS : lo + (t - n_pre) * KEYS;
@@ -478,9 +573,8 @@ __global__ __launch_bounds__(S::THREADS, S::D == 64 ? 3 : 2) void prefix_attn_ke
   __syncthreads();  // the images are free
 
   // Through LDS to whole rows.
-  const int rest = (T + S::ROWS - 1) / S::ROWS * H - full;
-  // partial rows: [split][item - full][row of the item]
-  const long base = ((long)split * rest + item - full) * S::ROWS;
+  // partial rows: [split][item - first_split][row of the item]
+  const long base = ((long)split * rest + item - first_split) * S::ROWS;
   const bool whole = parts == 1 && !DECODE;
   if (KW == 1 && whole) {
     __bf16* o_img = (__bf16*)smem + wave * 32 * D;
@@ -564,17 +658,17 @@ __global__ __launch_bounds__(S::THREADS, S::D == 64 ? 3 : 2) void prefix_attn_ke
 }
 
 // Joins the splits: a thread has four columns of a row.
-// An item is `rows` rows of one head; the items from `full` on were split.
+// An item is `rows` rows of one head; `rest` items were split.
 template <int D>
 __global__ __launch_bounds__(256) void prefix_join_kernel(
     const float* __restrict__ part_o, const float* __restrict__ part_ml,
-    __bf16* __restrict__ out, int T, int H, int rows, int full, int rest,
+    __bf16* __restrict__ out, int T, int H, int rows, int first_split, int rest,
     int splits, bool by_head) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const long pr = i / (D / 4);  // partial row: [item - full][row]
+  const long pr = i / (D / 4);  // partial row: [item - first_split][row]
   const int col = (int)(i % (D / 4)) * 4;
   if (pr >= (long)rest * rows) return;
-  const int item = full + (int)(pr / rows);
+  const int item = first_split + (int)(pr / rows);
   int tile, h;
   place(item, H, (T + rows - 1) / rows, by_head, tile, h);
   const long t = (long)tile * rows + pr % rows;

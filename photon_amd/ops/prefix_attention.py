@@ -14,6 +14,9 @@ tokens:
 Position i of a sequence's own tokens is position P + i of its text: the bias
 is -slope * (P + i - j) for key j of the prefix and -slope * (i - j) for its
 own key j <= i. Both run without gradients.
+
+A key whose weight is below 2^-150 of the row's largest adds nothing; on a GPU
+its value is then not looked at, so a NaN in it need not show.
 """
 
 from __future__ import annotations

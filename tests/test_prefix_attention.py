@@ -189,6 +189,36 @@ def test_packed_rows_larger(dev, D, lens, P, H):
 
 
 @gpu
+@pytest.mark.parametrize("H,D", [(64, 128), (100, 64)])
+@pytest.mark.parametrize("kind", ["alibi", "steep", "flat", "rising", "a far key counts", "a far key is NaN"])
+def test_far_keys_left_out(dev, H, D, kind):
+    """More items than one round of workgroups over a long prefix: tiles that
+    cannot count are not computed."""
+    lens, P = [90] * 12 + [1, 0, 30], 2601
+    qkv, prefix, slopes = make(dev, sum(lens), P, H, D, seed=H)
+    if kind == "steep":
+        slopes = torch.full_like(slopes, 1.0)
+    elif kind == "flat":
+        slopes = torch.zeros_like(slopes)
+    elif kind == "rising":
+        slopes = -0.1 * slopes
+    elif kind == "a far key counts":  # q . k / sqrt(d) stays below 2^9
+        prefix.view(P, 3, H, D)[0, 1, :, 5] = 1000.0
+    elif kind == "a far key is NaN":
+        prefix.view(P, 3, H, D)[70, 1, ::3, 5] = math.nan
+    got = prefix_attention_qkv(qkv, prefix, H, slopes, sequence_starts(lens, dev))
+    if kind == "a far key is NaN":
+        bad = got.view(-1, H, D).isnan()
+        assert bool(bad[:, ::3].all())
+        keep = torch.arange(H) % 3 != 0
+        sub = [x.view(-1, 3, H, D)[:, :, keep].flatten(1) for x in (qkv, prefix)]
+        want = exact(*sub, int(keep.sum()), slopes[keep], lens)
+        assert_near(got.view(-1, H, D)[:, keep].flatten(1), want)
+    else:
+        assert_near(got, exact(qkv, prefix, H, slopes, lens))
+
+
+@gpu
 def test_no_rows(dev):
     qkv, prefix, slopes = make(dev, 0, 9, 2, 64)
     assert prefix_attention_qkv(qkv, prefix, 2, slopes, sequence_starts([0, 0], dev)).shape == (0, 128)
