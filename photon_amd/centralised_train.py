@@ -60,6 +60,17 @@ def run_split_eval(cfg, trainer) -> dict:
     return out
 
 
+def _icl_needs_autocast(cfg, model, device) -> bool:
+    """fp32 weights on a GPU under flash attention, whose kernels take bf16;
+    every other model is evaluated in its weights' precision."""
+    llm = cfg["llm_config"]
+    attn = (llm.get("model") or {}).get("attn_config") or {}
+    return (torch.device(device).type == "cuda"
+            and str(llm.get("precision", "amp_bf16")) == "amp_bf16"
+            and str(attn.get("attn_impl", "flash")) == "flash"
+            and next(model.parameters()).dtype == torch.float32)
+
+
 def run_icl_eval(cfg, model, device) -> dict:
     """Config-gated ICL + gauntlet evaluation (icl_tasks_config /
     eval_gauntlet_config groups, both `empty` by default)."""
@@ -72,10 +83,8 @@ def run_icl_eval(cfg, model, device) -> dict:
     from .models import MPTCausalLM
 
     tok = load_tokenizer(icl_cfg.get("tokenizer_path"))
-    # fp32 weights on a GPU: the flash kernels take bf16
-    amp = (torch.device(device).type == "cuda"
-           and str(cfg["llm_config"].get("precision", "amp_bf16")) == "amp_bf16")
-    with torch.autocast("cuda", dtype=torch.bfloat16, enabled=amp):
+    with torch.autocast("cuda", dtype=torch.bfloat16,
+                        enabled=_icl_needs_autocast(cfg, model, device)):
         results = evaluate_icl_tasks(
             model, tasks, tok, device=device,
             max_seq_len=int(cfg["llm_config"].get("max_seq_len", 2048)),

@@ -129,7 +129,7 @@ def _greedy_generate(model, tok, prompt: str, device, max_len: int,
                      stop_strings: list[str] | None = None,
                      share_prefix: bool = False) -> str:
     ids = tok.encode(prompt)[-(max_len - max_new_tokens):]
-    if share_prefix and ids:
+    if share_prefix and ids and max_new_tokens > 0:
         return _generate_cached(model, tok, ids, max_new_tokens,
                                 stop_strings or [])
     x = torch.tensor([ids], dtype=torch.long, device=device)

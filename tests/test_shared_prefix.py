@@ -169,6 +169,24 @@ def test_eval_path_of_centralised_training(tmp_path):
     assert run_icl_eval(cfg, Wrapped(tiny(vocab=512)), "cpu") == got[False]
 
 
+def test_icl_precision():
+    """Autocast only where the flash kernels would refuse the weights."""
+    from photon_amd.centralised_train import _icl_needs_autocast
+
+    def needs(device="cuda", dtype=torch.float32, impl="flash", **llm):
+        cfg = {"llm_config": {"model": {"attn_config": {"attn_impl": impl}}, **llm}}
+        return _icl_needs_autocast(cfg, torch.nn.Linear(2, 2).to(dtype), device)
+
+    assert needs() and needs("cuda:0", precision="amp_bf16")
+    assert not (needs("cpu") or needs(dtype=torch.bfloat16) or needs(impl="torch") or needs(precision="fp32"))
+    assert _icl_needs_autocast({"llm_config": {}}, torch.nn.Linear(2, 2), "cuda")
+
+
+def test_no_tokens_to_generate():
+    m, tok = tiny(vocab=512), ByteTokenizer()
+    assert all(_greedy_generate(m, tok, "abc", "cpu", 50, 0, share_prefix=s) == "" for s in (False, True))
+
+
 def test_emb_scale_in_the_model():
     """emb_scale is read from the configuration, survives a resize, and 1.0
     leaves the model as it was."""
