@@ -48,7 +48,8 @@ def clip_grads_(grads, max_norm: float) -> tuple[torch.Tensor, torch.Tensor]:
     scale = max_norm / (total + 1e-6)
     if not scale >= 1.0:
         for g in grads:
-            g.copy_(g.float() * scale)
+            wide = g.double() if g.dtype == torch.float64 else g.float()
+            g.copy_(wide * scale)
     return total, norms
 
 

@@ -59,6 +59,16 @@ def test_plain_path(max_norm):
     assert torch.equal(t2, total) and torch.equal(n2, norms)
 
 
+def test_64_bit_gradients_stay_64_bit():
+    g = torch.randn(100, dtype=torch.float64)
+    want = g * float((0.5 / (g.norm() + 1e-6)))
+    clip_grads_([g], 0.5)
+    # the factor is rounded to fp32, the same for all: the ratios are exact
+    ratio = g / want
+    assert (ratio / ratio[0] - 1).abs().max() <= 2.0**-50
+    assert abs(ratio[0] - 1) <= 4 * 2.0**-24
+
+
 def test_refusals_and_empty():
     with pytest.raises(ValueError, match="max_norm"):
         clip_grads_([torch.ones(2)], -1.0)
