@@ -177,11 +177,11 @@ torch::Tensor prefix_attention(torch::Tensor qkv, torch::Tensor prefix, long H,
   // long as before) over a long prefix. 32 heads of 128, 4000 rows: 237 us
   // without and 195 with over 4000 keys, 145 and 143 over 2000, 93 and 94 over
   // 1000; 2000 rows (one round) over 4000 keys 121 and 120.
-  if (c.first_split > 0 && a.P >= 2500) {
+  if (c.first_split > 0 && a.P >= 2500 && a.P < (1 << 28)) {  // (grid.x)
     const int tiles = (a.P + NORM_KEYS - 1) / NORM_KEYS;
     norms = torch::empty({(long)a.H * tiles}, qkv.options().dtype(at::kFloat));
     auto fn = a.D == 64 ? key_norms_kernel<64> : key_norms_kernel<128>;
-    hipLaunchKernelGGL(fn, dim3(a.H, tiles), dim3(256), 0, cur_stream(),
+    hipLaunchKernelGGL(fn, dim3(tiles, a.H), dim3(256), 0, cur_stream(),
                        (const __bf16*)a.prefix.data_ptr() + (long)a.H * a.D,
                        a.prefix.stride(0), norms.data_ptr<float>(), a.P);
   }

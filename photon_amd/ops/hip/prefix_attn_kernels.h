@@ -140,7 +140,7 @@ __global__ __launch_bounds__(256) void key_norms_kernel(
     int P) {
   constexpr int L = D / 8, G = 256 / L;
   __shared__ float s_max[4];
-  const int h = blockIdx.x, tile = blockIdx.y;
+  const int tile = blockIdx.x, h = blockIdx.y;
   const int g = threadIdx.x / L, c = threadIdx.x % L * 8;
   const __bf16* at = pk + (long)h * D + c;
   float top = 0.f;
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(256) void key_norms_kernel(
 #pragma unroll
     for (int w = 1; w < 4; ++w)
       top = __builtin_elementwise_maximum(top, s_max[w]);
-    norms[(long)h * gridDim.y + tile] = top;
+    norms[(long)h * gridDim.x + tile] = top;
   }
 }
 

@@ -16,7 +16,9 @@ is -slope * (P + i - j) for key j of the prefix and -slope * (i - j) for its
 own key j <= i. Both run without gradients.
 
 A key whose weight is below 2^-150 of the row's largest adds nothing; on a GPU
-its value is then not looked at, so a NaN in it need not show.
+its value is then not looked at, so a NaN in it need not show. The kernels
+take scores and biases up to 2^28 (their weights are differences of fp32 values,
+which are whole numbers beyond 2^24).
 """
 
 from __future__ import annotations

@@ -412,3 +412,47 @@ def test_long_prefix_offsets_pass_32_bits(dev):
     slopes = torch.full_like(slopes, 1e-3)
     got = prefix_attention_qkv(qkv, prefix, H, slopes, sequence_starts([3], dev))
     assert_near(got, exact(qkv, small, H, slopes, [3]))
+
+
+@gpu
+def test_many_rows_over_millions_of_keys(dev):
+    """Slope 1: only the last keys count, as over a prefix of these alone; and
+    one that is far and large enough to be all that counts."""
+    H, D, P, near = 1, 64, 4_200_000, 1000
+    lens = [64] * 1540
+    g = torch.Generator(device=dev).manual_seed(5)
+    prefix = torch.randn(P, 3 * D, generator=g, device=dev, dtype=BF16)
+    qkv = torch.randn(sum(lens), 3 * D, generator=g, device=dev, dtype=BF16)
+    slopes, starts = torch.ones(1, device=dev), sequence_starts(lens, dev)
+    got = prefix_attention_qkv(qkv, prefix, H, slopes, starts)
+    assert_near(got[:192], exact(qkv[:192], prefix[-near:], H, slopes, lens[:3]))
+    want = prefix_attention_qkv(qkv, prefix[-near:], H, slopes, starts)
+    # both are off by what one call is allowed: weights, then the result
+    room = 2 * (2.0**-8 + 2.0**-9) * 6.0 + 2.0**-7 * want.float().abs()
+    assert bool(((got.float() - want.float()).abs() <= room).all())
+    prefix[0, D + 5] = 2.0**30
+    got = prefix_attention_qkv(qkv, prefix, H, slopes, starts)
+    hit, miss = qkv[:, 5] > 0.25, qkv[:, 5] < 0
+    # one weight p counts: round(p) * v / p with |round(p) / p - 1| <= 2^-8
+    # (scores of 2^28 leave p anywhere within 2^64), then the result's rounding
+    v = prefix[0, 2 * D:].float()
+    assert bool(((got[hit].float() - v).abs() <= (2.0**-8 + 2.0**-8 * (1 + 2.0**-8)) * v.abs()).all())
+    assert bool(((got - want).float().abs() <= room)[miss].all())
+
+
+@gpu
+def test_graph_of_many_rows(dev):
+    """The three kernels of a large call in a graph, on new inputs."""
+    H, D, lens, P = 64, 128, [100] * 11, 2600
+    qkv, prefix, slopes = make(dev, sum(lens), P, H, D)
+    starts = sequence_starts(lens, dev)
+    prefix_attention_qkv(qkv, prefix, H, slopes, starts)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = prefix_attention_qkv(qkv, prefix, H, slopes, starts)
+    for i in range(1, 4):
+        qkv.mul_(-1.0)
+        prefix.mul_(1.25)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, prefix_attention_qkv(qkv, prefix, H, slopes, starts))
