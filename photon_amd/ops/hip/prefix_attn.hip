@@ -227,19 +227,34 @@ torch::Tensor prefix_attention_decode(torch::Tensor qkv, torch::Tensor prefix,
   if (B == 0) return out;
   Cut c{};
   c.rows = 1;
-  if (a.P > 0) c = cut(B, a.H, a.D, a.P, true);
+  // Up to a workgroup a CU each is a large one, which also attends a short
+  // prefix by itself: there is next to nothing to share, and one kernel is the
+  // shorter chain. 12 heads of 64 over 700 keys, 1 to 16 sequences: 7.4 us, and
+  // 10.6 in two kernels; 32 heads of 128, 1 to 4 sequences, over 1000 keys 10.2
+  // and 13.6, over 2000 keys 17 and 16; 16 sequences of them over 700 keys 16.9
+  // and 13.8. Caches of 4000 own keys, 32 heads of 128: 30 us, and 71 in small
+  // workgroups.
+  const bool large = B * a.H <= 256;
+  const bool direct = large && a.P > 0 && (long)a.P * a.D <= 160000;
+  if (a.P > 0 && !direct) c = cut(B, a.H, a.D, a.P, true);
   const Partial part(c, a.D, qkv);
-  if (a.P > 0)
+  if (a.P > 0 && !direct)
     launch<true>(a.qkv, a.prefix, a.H, a.D, a.slopes, a.info, nullptr,
                  nullptr, part.o,
                  part.ml, a.T, a.P, c);
-  auto own = a.D == 64 ? decode_own_kernel<64> : decode_own_kernel<128>;
-  hipLaunchKernelGGL(own, dim3(a.H, (unsigned)B), dim3(OWN_BLOCK), 0,
+  const __bf16* pk = (const __bf16*)a.prefix.data_ptr() + (long)a.H * a.D;
+  auto own = large ? (a.D == 64 ? decode_own_kernel<64, LARGE_BLOCK>
+                                : decode_own_kernel<128, LARGE_BLOCK>)
+                   : (a.D == 64 ? decode_own_kernel<64, OWN_BLOCK>
+                                : decode_own_kernel<128, OWN_BLOCK>);
+  hipLaunchKernelGGL(own, dim3(a.H, (unsigned)B),
+                     dim3(large ? LARGE_BLOCK : OWN_BLOCK), 0,
                      cur_stream(), (const __bf16*)a.qkv.data_ptr(),
                      a.qkv.stride(0), (__bf16*)cache.data_ptr(),
                      cache.stride(0), cache.stride(1), cache.stride(2),
                      cache.stride(3), a.slopes.data_ptr<float>(),
-                     a.info.data_ptr<int>(), part.o, part.ml,
+                     a.info.data_ptr<int>(), pk, pk + (long)a.H * a.D,
+                     a.prefix.stride(0), direct ? a.P : 0, part.o, part.ml,
                      (__bf16*)out.data_ptr(), a.H, (int)cache.size(1), c.rows,
                      c.items, c.splits);
   cache.unsafeGetTensorImpl()->bump_version();  // written in place

@@ -31,7 +31,8 @@
 // CUs'; the rest is waiting, at 1.6 waves a SIMD of 2. Few rows (93 over 1507, 16
 // heads of 128): 12 us and 4 for the join, a chain of latencies. One new token
 // for each of 64 sequences over 3967 keys and caches of 512, 32 heads of 128: 20
-// us for the prefix (66 MB) and 60 for the caches (267 MB, 4.4 TB/s).
+// us for the prefix (66 MB) and 60 for the caches (267 MB, 4.4 TB/s); for one
+// sequence over 701 keys, 12 heads of 64, 7 us.
 
 #pragma once
 
@@ -699,19 +700,23 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(
 // the cache, attends the sequence's own keys and joins what the prefix gave.
 // D / 8 lanes hold a key's 8 columns each, all groups of the block stride
 // over the keys with a running maximum and sum of their own.
+// Where there are few workgroups each is a large one, and may attend `direct`
+// keys of the prefix as well (all of them; no partial rows then).
 constexpr int OWN_BLOCK = 256;
-template <int D>
-__global__ __launch_bounds__(OWN_BLOCK) void decode_own_kernel(
+constexpr int LARGE_BLOCK = 1024;
+template <int D, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void decode_own_kernel(
     const __bf16* __restrict__ qkv, long q_rs, __bf16* __restrict__ cache,
     long c_bs, long c_ss, long c_ks, long c_hs,
     const float* __restrict__ slopes, const int* __restrict__ held,
-    const float* __restrict__ part_o, const float* __restrict__ part_ml,
-    __bf16* __restrict__ out, int H, int slots, int rows, int items,
-    int splits) {
+    const __bf16* __restrict__ pk, const __bf16* __restrict__ pv, long p_rs,
+    int direct, const float* __restrict__ part_o,
+    const float* __restrict__ part_ml, __bf16* __restrict__ out, int H,
+    int slots, int rows, int items, int splits) {
   constexpr int L = D / 8;               // lanes a key
-  constexpr int G = OWN_BLOCK / L;       // keys at a time
-  __shared__ float s_o[OWN_BLOCK / 64][D];
-  __shared__ float s_m[OWN_BLOCK / 64], s_l[OWN_BLOCK / 64];
+  constexpr int G = BLOCK / L;           // keys at a time
+  __shared__ float s_o[BLOCK / 64][D];
+  __shared__ float s_m[BLOCK / 64], s_l[BLOCK / 64];
   const int h = blockIdx.x;
   const int b = blockIdx.y;
   const int tid = threadIdx.x;
@@ -757,46 +762,54 @@ __global__ __launch_bounds__(OWN_BLOCK) void decode_own_kernel(
   float m = -1e30f, l = 0.f, o[8] = {};
   // U keys at a time, all their loads in flight together and one rescaling
   constexpr int U = 4;
-  for (int i0 = g; i0 <= n; i0 += U * G) {
-    bf16x8 kv[U], vv[U];
+  // keys 0 .. count - 1, which lie `stored` rows of stride `rs` behind k0 and
+  // v0; the rest (the new one) come from registers. Key i is gap - i away.
+  auto attend = [&](int count, int stored, const __bf16* k0, const __bf16* v0,
+                    long rs, int gap) {
+    for (int i0 = g; i0 < count; i0 += U * G) {
+      bf16x8 kv[U], vv[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * G;
-      kv[u] = new_k;  // the new ones from registers
-      vv[u] = new_v;
-      if (i < n) {
-        kv[u] = *(const bf16x8*)(ck + (long)i * c_ss + c);
-        vv[u] = *(const bf16x8*)(cv + (long)i * c_ss + c);
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * G;
+        kv[u] = new_k;
+        vv[u] = new_v;
+        if (i < stored) {
+          kv[u] = *(const bf16x8*)(k0 + (long)i * rs + c);
+          vv[u] = *(const bf16x8*)(v0 + (long)i * rs + c);
+        }
+      }
+      float w[U];
+      float m_new = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x = fmaf(qf[j], (float)kv[u][j], x);
+#pragma unroll
+        for (int off = L / 2; off > 0; off >>= 1) x += __shfl_xor(x, off, WAVE);
+        const int i = i0 + u * G;
+        w[u] = i < count ? x - slope2 * (float)(gap - i) : -INFINITY;
+        m_new = fmaxf(m_new, w[u]);
+      }
+      const float a = exp2_fast(m - m_new);
+      m = m_new;
+      l *= a;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] *= a;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i0 + u * G < count) {  // a value behind the last is not touched
+          const float p = exp2_fast(w[u] - m);
+          l += p;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = fmaf(p, (float)vv[u][j], o[j]);
+        }
       }
     }
-    float w[U];
-    float m_new = m;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float x = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x = fmaf(qf[j], (float)kv[u][j], x);
-#pragma unroll
-      for (int off = L / 2; off > 0; off >>= 1) x += __shfl_xor(x, off, WAVE);
-      const int i = i0 + u * G;
-      w[u] = i <= n ? x - slope2 * (float)(n - i) : -INFINITY;
-      m_new = fmaxf(m_new, w[u]);
-    }
-    const float a = exp2_fast(m - m_new);
-    m = m_new;
-    l *= a;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] *= a;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i0 + u * G <= n) {  // a value behind the new one is not touched
-        const float p = exp2_fast(w[u] - m);
-        l += p;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = fmaf(p, (float)vv[u][j], o[j]);
-      }
-    }
-  }
+  };
+  if (direct > 0)
+    attend(direct, direct, pk + (long)h * D, pv + (long)h * D, p_rs, direct + n);
+  attend(n + 1, n, ck, cv, c_ss, n);
   // the wave's groups, then the block's waves
 #pragma unroll
   for (int off = L; off < WAVE; off <<= 1) {
@@ -828,10 +841,10 @@ __global__ __launch_bounds__(OWN_BLOCK) void decode_own_kernel(
   for (int s = EARLY; s < splits; ++s)
     M = fmaxf(M, part_ml[(s * stride + pr) * 2]);
 #pragma unroll
-  for (int w = 0; w < OWN_BLOCK / 64; ++w) M = fmaxf(M, s_m[w]);
+  for (int w = 0; w < BLOCK / 64; ++w) M = fmaxf(M, s_m[w]);
   float sum = 0.f, acc = 0.f;
 #pragma unroll
-  for (int w = 0; w < OWN_BLOCK / 64; ++w) {
+  for (int w = 0; w < BLOCK / 64; ++w) {
     const float a = exp2_fast(s_m[w] - M);
     sum += a * s_l[w];
     acc += a * s_o[w][tid];

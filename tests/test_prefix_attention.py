@@ -310,6 +310,8 @@ def test_starts_out_of_range_stay_inside(dev, H):
     (1, 0, 1, 3), (1, 701, 24, 3), (3, 64, 7, 3), (33, 65, 40, 3), (70, 300, 130, 3), (2, 5, 700, 3),
     (1, 3000, 5, 1),  # more splits than are asked for early
     (400, 130, 9, 12), (130, 1, 3, 40),  # more than 128 items of 32 rows
+    # a workgroup a CU each, and one more; the longest prefix that one attends
+    (16, 40, 6, 16), (257, 40, 6, 1), (2, 1250, 300, 4), (2, 1251, 300, 4), (1, 2500, 2000, 2), (1, 2501, 3, 2),
 ])
 def test_decode(dev, D, B, P, slots, H):
     """Against the packed form's definition, with NaN in every unused slot."""
