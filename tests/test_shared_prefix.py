@@ -187,6 +187,26 @@ def test_no_tokens_to_generate():
     assert all(_greedy_generate(m, tok, "abc", "cpu", 50, 0, share_prefix=s) == "" for s in (False, True))
 
 
+def inference_mode_matches(m, dev):
+    """Scores and steps, inside inference mode and with a model made outside."""
+    def run():
+        shared = SharedPrefix(m, list(range(20)))
+        shared.begin(2, 3)
+        outs = [shared.score([[5, 6, 7], [8]])]
+        outs += [shared.step(torch.tensor([i, i + 1], device=dev)) for i in range(3)]
+        return torch.cat([shared.logits(x) for x in outs])
+
+    with torch.no_grad():
+        want = run()
+    with torch.inference_mode():
+        got = run()
+        assert torch.equal(got, want)
+
+
+def test_inference_mode():
+    inference_mode_matches(tiny(), "cpu")
+
+
 def test_emb_scale_in_the_model():
     """emb_scale is read from the configuration, survives a resize, and 1.0
     leaves the model as it was."""
@@ -225,6 +245,11 @@ def test_gpu_scores_match_whole_sequences(dev, d, heads, weights):
     else:
         with torch.autocast("cuda", dtype=torch.bfloat16):
             assert_scores(m, prefix, SEQS, 0.1)
+
+
+@gpu
+def test_gpu_inference_mode(dev):
+    inference_mode_matches(tiny("flash", 256, 4).to(dev, torch.bfloat16), dev)
 
 
 @gpu
