@@ -151,5 +151,15 @@ def _plain(qkv, prefix_qkv, n_heads, slopes, starts):
         q @ pk.transpose(1, 2) * scale - slope * far,
         (q @ k.transpose(1, 2) * scale - slope * near).masked_fill(~seen, -math.inf),
     ], -1)
-    o = torch.softmax(w, -1) @ torch.cat([pv, v], 1)
+    # A weight of zero does not hide an infinity or NaN: values that are not
+    # finite are taken out and added for the rows that see them (a NaN as an
+    # infinity of either sign). On a GPU without looking whether there are any.
+    finite = v.isfinite()
+    every = v.device.type == "cpu" and bool(finite.all())
+    o = torch.softmax(w, -1) @ torch.cat([pv, v.where(finite, 0.0)], 1)
+    if not every:
+        sight = seen.to(wide)
+        for sign in (math.inf, -math.inf):
+            bad = (v.isnan() | (v == sign)).to(wide)
+            o = torch.where(sight @ bad > 0, o + sign, o)
     return o.transpose(0, 1).reshape(T, -1).to(qkv.dtype)

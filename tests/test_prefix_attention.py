@@ -105,6 +105,49 @@ def test_plain_decode_steps_match_packed_rows():
         prefix_attention_decode(qkv[:3], prefix, H, slopes, cache, held + 3)
 
 
+def plain_keeps_bad_values(dev):
+    """The plain path, as the kernels: what is not finite in a key or value
+    reaches the rows that see it and no others."""
+    H, D, lens, P = 2, 8, [3, 0, 5, 2], 4
+    F64 = torch.float64
+    qkv, prefix, slopes = make(dev, 10, P, H, D, F64)
+    starts = sequence_starts(lens, dev)
+    out, mag = (x.to(dev) for x in exact(qkv, prefix, H, slopes, lens))
+    sees = torch.arange(10, device=dev).ge(5) & torch.arange(10, device=dev).lt(8)
+    for bad in (math.nan, math.inf, -math.inf):
+        x = qkv.clone()
+        x[5, 2 * H * D + 3] = bad  # the third of the second sequence's five
+        got = prefix_attention_qkv(x, prefix, H, slopes, starts, impl="torch")
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[sees, 3] = True
+        assert bool(((got - out).abs() <= 1e-12 * mag)[~hit].all())
+        assert bool((got[hit].isnan() if math.isnan(bad) else got[hit] == bad).all())
+        x = qkv.clone()
+        x[5, H * D + 3] = bad  # of its key: one head, and a weight may be zero
+        got = prefix_attention_qkv(x, prefix, H, slopes, starts, impl="torch")
+        hit.zero_()[sees, :D] = True
+        assert bool(((got - out).abs() <= 1e-12 * mag)[~hit].all())
+    x = qkv.clone()
+    x[3, 2 * H * D], x[5, 2 * H * D] = math.inf, -math.inf  # NaN for who sees both
+    got = prefix_attention_qkv(x, prefix, H, slopes, starts, impl="torch")[:, 0]
+    assert got[3:5].eq(math.inf).all() and got[5:8].isnan().all() and got[[0, 1, 2, 8, 9]].isfinite().all()
+    # single tokens: a cached value of one sequence, and a new one
+    cache = torch.randn(3, 4, 2, H, D, generator=torch.Generator().manual_seed(3)).to(dev, F64)
+    held = torch.tensor([2, 3, 0], dtype=torch.int32, device=dev)
+    new = qkv[:3].clone()
+    want = prefix_attention_decode(new, prefix, H, slopes, cache.clone(), held, impl="torch")
+    cache[0, 1, 1, 1, 2] = math.inf
+    new[2, 2 * H * D] = math.nan
+    got = prefix_attention_decode(new, prefix, H, slopes, cache, held, impl="torch")
+    assert got[0, D + 2] == math.inf and got[2, 0].isnan()
+    got[0, D + 2], got[2, 0] = want[0, D + 2], want[2, 0]
+    assert (got - want).abs().max() <= 1e-12
+
+
+def test_plain_path_keeps_bad_values_in_their_sequence():
+    plain_keeps_bad_values("cpu")
+
+
 def refusals(dev):
     H, D = 2, 64
     qkv, prefix, slopes = make(dev, 5, 9, H, D)
@@ -148,6 +191,11 @@ def check(dev, lens, P, H, D, seed=0):
     got = prefix_attention_qkv(qkv, prefix, H, slopes, sequence_starts(lens, dev))
     assert got.dtype == BF16 and got.shape == (sum(lens), H * D)
     assert_near(got, exact(qkv, prefix, H, slopes, lens))
+
+
+@gpu
+def test_plain_path_on_a_gpu_keeps_bad_values_in_their_sequence(dev):
+    plain_keeps_bad_values(dev)
 
 
 @gpu
