@@ -12,6 +12,15 @@ inline hipStream_t cur_stream() {
   return at::hip::getCurrentHIPStream().stream();
 }
 
+// Before the kernels that write `t` in place: counting up its version, which
+// they have to do, fails where this is not so.
+inline void check_writable(const torch::Tensor& t, const char* name,
+                           const char* what) {
+  TORCH_CHECK(!t.is_inference() || c10::InferenceMode::is_enabled(), name,
+              ": ", what, " was made in inference mode and cannot be written "
+              "outside of it");
+}
+
 #define DISPATCH_DTYPE(TENSOR, NAME, ...)                              \
   if ((TENSOR).scalar_type() == at::kBFloat16) {                       \
     using scalar_t = unsigned short;                                   \

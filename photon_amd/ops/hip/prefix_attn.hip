@@ -223,6 +223,7 @@ torch::Tensor prefix_attention_decode(torch::Tensor qkv, torch::Tensor prefix,
               "aligned to 16 bytes");
   TORCH_CHECK(B < 65536 && cache.size(1) < (1L << 30), name,
               ": too many sequences or slots");
+  check_writable(cache, name, "the cache");
   auto out = torch::empty({B, (long)a.H * a.D}, qkv.options());
   if (B == 0) return out;
   Cut c{};

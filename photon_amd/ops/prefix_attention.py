@@ -116,6 +116,9 @@ def prefix_attention_decode(
                          f"{', '.join(map(str, want))}], got {tuple(cache.shape)}")
     if cache.dtype != qkv.dtype or cache.device != qkv.device:
         raise ValueError(f"{name}: cache must have qkv's dtype and device")
+    if cache.is_inference() and not torch.is_inference_mode_enabled():
+        raise RuntimeError(f"{name}: the cache was made in inference mode and "
+                           "cannot be written outside of it")
     B = qkv.shape[0]
     rows, slots = held.long(), cache.shape[1]
     if bool(((rows < 0) | (rows >= slots)).any()):

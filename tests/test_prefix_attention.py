@@ -178,6 +178,26 @@ def test_refusals():
     refusals("cpu")
 
 
+def refused_cache_stays(dev):
+    """A cache made in inference mode cannot be written outside of it: the
+    call says so and leaves it as it is."""
+    H, D = 2, 64
+    qkv, prefix, slopes = make(dev, 3, 9, H, D)
+    held = torch.zeros(3, dtype=torch.int32, device=dev)
+    with torch.inference_mode():
+        cache = torch.ones(3, 4, 2, H, D, dtype=BF16, device=dev)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="cache was made in inference mode"):
+        prefix_attention_decode(qkv, prefix, H, slopes, cache, held)
+    assert bool((cache == 1).all())
+    with torch.inference_mode():
+        prefix_attention_decode(qkv, prefix, H, slopes, cache, held)
+    assert torch.equal(cache[:, 0], qkv[:, H * D:].view(3, 2, H, D)) and bool((cache[:, 1:] == 1).all())
+
+
+def test_refused_cache_stays():
+    refused_cache_stays("cpu")
+
+
 # -- GPU --------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def dev():
@@ -196,6 +216,11 @@ def check(dev, lens, P, H, D, seed=0):
 @gpu
 def test_plain_path_on_a_gpu_keeps_bad_values_in_their_sequence(dev):
     plain_keeps_bad_values(dev)
+
+
+@gpu
+def test_gpu_refused_cache_stays(dev):
+    refused_cache_stays(dev)
 
 
 @gpu
