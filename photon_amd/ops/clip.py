@@ -44,6 +44,9 @@ def clip_grads_(grads, max_norm: float) -> tuple[torch.Tensor, torch.Tensor]:
     if use_hip(grads[0]):
         total, norms = hip_ext().clip_grads(grads, max_norm)
         return total, norms
+    if not torch.is_inference_mode_enabled() and any(g.is_inference() for g in grads):
+        raise RuntimeError("clip_grads_: a gradient was made in inference mode "
+                           "and cannot be written outside of it")
     total, norms = tensor_norms(grads)
     scale = max_norm / (total + 1e-6)
     if not scale >= 1.0:

@@ -86,6 +86,25 @@ def test_parameter_listed_twice_counts_once():
     assert torch.allclose(p.grad, torch.full((4,), 1.5))
 
 
+def refused_gradients_stay(dev):
+    """One gradient made in inference mode: outside of it none is scaled."""
+    plain = [torch.full((9,), 3.0, device=dev), torch.full((4, 6), 2.0, device=dev)[:, ::2]]
+    with torch.inference_mode():
+        made = torch.full((5,), 4.0, device=dev)
+    grads = [plain[0], made, plain[1]]
+    with pytest.raises(RuntimeError, match="gradient was made in inference mode"):
+        clip_grads_(grads, 0.5)
+    assert all(bool((g == x).all()) for g, x in zip(grads, (3.0, 4.0, 2.0)))
+    before = [g.clone() for g in grads]
+    with torch.inference_mode():
+        total, norms = clip_grads_([made], 0.5)
+    assert_clipped([made], before[1:2], total, norms, 0.5)
+
+
+def test_refused_gradients_stay():
+    refused_gradients_stay("cpu")
+
+
 def test_optimizer_monitor_matches_the_loop():
     from types import SimpleNamespace
 
@@ -183,6 +202,11 @@ def test_strided_gradients(dev):
     assert_clipped(grads, before, total, norms, 1.0)
     assert torch.equal(b[:, 3::4], rest_b[:, 3::4])
     assert not torch.equal(a, rest_a)
+
+
+@gpu
+def test_gpu_refused_gradients_stay(dev):
+    refused_gradients_stay(dev)
 
 
 @gpu
