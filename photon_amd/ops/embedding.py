@@ -30,7 +30,7 @@ def embedding(
     """Rows ``ids`` (int64 or int32, any shape) of ``table`` [V, D] (fp32 or
     bf16), times ``scale``, as ``out_dtype`` (default: the table's).
 
-    Differentiable once in ``table``. An id outside [0, V) raises IndexError
+    Differentiable once in ``table``; on the GPU not in forward mode. An id outside [0, V) raises IndexError
     on the CPU; on the GPU, where looking would wait for the device, its row
     is NaN and it has no gradient."""
     out_dtype = out_dtype or table.dtype

@@ -709,6 +709,7 @@ class EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "embedding: a second derivative is not supported "
                 "(create_graph=True)");
+    check_no_tangent(grads[0], "embedding");
     auto ids = ctx->get_saved_variables()[0];
     auto dw = embedding_bwd(grads[0], ids, ctx->saved_data["rows"].toInt(),
                             ctx->saved_data["scale"].toDouble(),
@@ -739,6 +740,7 @@ torch::Tensor embedding(torch::Tensor ids, torch::Tensor w, double scale,
   TORCH_CHECK(ids.device() == w.device(), "embedding: ids on ", ids.device(),
               ", table on ", w.device());
   TORCH_CHECK(known_dtype(out_dtype), "embedding: output must be fp32 or bf16");
+  check_no_tangent(w, "embedding");
   if (w.requires_grad() && at::GradMode::is_enabled())
     return EmbeddingFn::apply(w, ids, scale, (int64_t)out_dtype);
   return embedding_fwd(ids, w, scale, out_dtype);

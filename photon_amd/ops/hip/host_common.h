@@ -21,6 +21,13 @@ inline void check_writable(const torch::Tensor& t, const char* name,
               "outside of it");
 }
 
+// A kernel does not carry forward-mode tangents: without this they would be
+// dropped in silence.
+inline void check_no_tangent(const torch::Tensor& t, const char* name) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), name,
+                              ": forward-mode derivatives are not supported");
+}
+
 #define DISPATCH_DTYPE(TENSOR, NAME, ...)                              \
   if ((TENSOR).scalar_type() == at::kBFloat16) {                       \
     using scalar_t = unsigned short;                                   \

@@ -10,6 +10,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from photon_amd.ops.embedding import FusedEmbedding, embedding
 
@@ -202,6 +203,23 @@ def test_gpu_refusals(dev):
     y = embedding(ids, w)
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(y.square().sum(), w, create_graph=True)
+
+
+@gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(dev, grad):
+    """A tangent of the table, or of the output's gradient, is not dropped."""
+    w = torch.randn(10, 16, device=dev, requires_grad=grad)
+    ids = torch.tensor([3, 3, 9], device=dev)
+    with fwAD.dual_level():
+        with pytest.raises(NotImplementedError, match="embedding: forward-mode"):
+            embedding(ids, fwAD.make_dual(w, torch.ones_like(w)))
+        if grad:
+            y = embedding(ids, w)
+            dy = fwAD.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(NotImplementedError, match="embedding: forward-mode"):
+                torch.autograd.grad(y, w, dy)
+    assert torch.equal(embedding(ids, w), w[ids])
 
 
 @gpu
