@@ -15,6 +15,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import hip_ext, use_hip
 
@@ -46,9 +47,22 @@ def embedding(
     return y.to(out_dtype)
 
 
+def _kernel_sees(w: torch.Tensor) -> bool:
+    """A plain table with whole rows, outside of forward mode, ``torch.func``
+    transforms and tracing: none of them sees what a kernel does."""
+    return (type(w) in (torch.Tensor, nn.Parameter)
+            and (w.stride(1) == 1 or w.shape[1] <= 1)
+            and forward_ad._current_level < 0
+            and not torch._C._are_functorch_transforms_active()
+            and not torch.jit.is_tracing()
+            and not torch.compiler.is_compiling())
+
+
 class FusedEmbedding(nn.Embedding):
     """``nn.Embedding`` whose rows come out scaled, and in the autocast dtype
-    where autocast is on. ``impl="torch"`` keeps torch's lookup and gradient."""
+    where autocast is on. ``impl="torch"`` keeps torch's lookup and gradient,
+    which also serve where the kernel cannot (:func:`_kernel_sees`), but for
+    second derivatives, which only ``impl="torch"`` has on a GPU."""
 
     def __init__(self, num_embeddings: int, embedding_dim: int,
                  scale: float = 1.0, impl: str = "fused", **kw):
@@ -67,7 +81,7 @@ class FusedEmbedding(nn.Embedding):
         if torch.is_autocast_enabled(kind):
             out_dtype = torch.get_autocast_dtype(kind)
         fused = self.impl == "fused" and w.dtype in _FLOATS \
-            and out_dtype in _FLOATS
+            and out_dtype in _FLOATS and _kernel_sees(w)
         if fused:
             return embedding(ids, w, self.scale, out_dtype)
         y = F.embedding(ids, w)

@@ -80,6 +80,41 @@ def test_module_matches_nn_embedding_on_cpu():
     assert torch.equal(s(ids), b(ids) * 2.5)
 
 
+def module_takes_what_nn_embedding_takes(dev):
+    """Transforms, forward mode, tracing, tables that are not rows of one
+    buffer: the module's results are nn.Embedding's times the scale."""
+    torch.manual_seed(2)
+    a, b = FusedEmbedding(11, 6, scale=2.0).to(dev), torch.nn.Embedding(11, 6).to(dev)
+    b.load_state_dict(a.state_dict())
+    w = a.weight.detach()
+    ids = torch.tensor([[3, 0, 3], [10, 7, 1]], device=dev)
+
+    def apply(m, table):
+        return torch.func.functional_call(m, {"weight": table}, (ids,))
+
+    tables = torch.stack([w, w + 1.0])
+    assert torch.equal(torch.func.vmap(lambda t: apply(a, t))(tables),
+                       2.0 * torch.func.vmap(lambda t: apply(b, t))(tables))
+    grad = torch.func.grad(lambda t: apply(a, t).square().sum())(w)
+    assert torch.equal(grad, 4.0 * torch.func.grad(lambda t: apply(b, t).square().sum())(w))
+    y, t = torch.func.jvp(lambda t: apply(a, t), (w,), (w.cos(),))
+    assert torch.equal(y, 2.0 * w[ids]) and torch.equal(t, 2.0 * w.cos()[ids])
+    with fwAD.dual_level():
+        y, t = fwAD.unpack_dual(apply(a, fwAD.make_dual(w, w.cos())))
+        assert torch.equal(y, 2.0 * w[ids]) and torch.equal(t, 2.0 * w.cos()[ids])
+    other = ids.flip(0)
+    assert torch.equal(torch.jit.trace(a, (ids,))(other), 2.0 * w[other])
+    table = w.t().contiguous().t().requires_grad_()  # columns, not rows, in one piece
+    y = apply(a, table)
+    assert torch.equal(y, 2.0 * w[ids])
+    assert torch.equal(torch.autograd.grad(y.square().sum(), table)[0], grad)
+    assert torch.equal(a(ids), 2.0 * w[ids])
+
+
+def test_module_takes_what_nn_embedding_takes():
+    module_takes_what_nn_embedding_takes("cpu")
+
+
 # -- GPU --------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def dev():
@@ -184,6 +219,11 @@ def test_strides_and_alignment(dev):
         assert_grad(g, ids, dy, 1.0)
     with pytest.raises(RuntimeError, match="contiguous"):
         embedding(ids, base.t())
+
+
+@gpu
+def test_gpu_module_takes_what_nn_embedding_takes(dev):
+    module_takes_what_nn_embedding_takes(dev)
 
 
 @gpu
