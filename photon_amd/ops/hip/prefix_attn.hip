@@ -110,6 +110,7 @@ Args check(const char* name, const torch::Tensor& qkv,
                         qkv.size(1) % (3 * H) == 0,
                     name, ": qkv must be [rows, 3 * n_heads * d], got ",
                     qkv.sizes(), " for ", H, " heads");
+  for (const auto* t : {&qkv, &prefix, &slopes}) check_no_tangent(*t, name);
   const long width = qkv.size(1), D = width / (3 * H);
   TORCH_CHECK_VALUE(prefix.dim() == 2 && prefix.size(1) == width, name,
                     ": prefix_qkv must be [P, ", width, "], got ",
@@ -224,6 +225,7 @@ torch::Tensor prefix_attention_decode(torch::Tensor qkv, torch::Tensor prefix,
   TORCH_CHECK(B < 65536 && cache.size(1) < (1L << 30), name,
               ": too many sequences or slots");
   check_writable(cache, name, "the cache");
+  check_no_tangent(cache, name);
   auto out = torch::empty({B, (long)a.H * a.D}, qkv.options());
   if (B == 0) return out;
   Cut c{};

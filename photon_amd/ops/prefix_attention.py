@@ -13,7 +13,8 @@ tokens:
 
 Position i of a sequence's own tokens is position P + i of its text: the bias
 is -slope * (P + i - j) for key j of the prefix and -slope * (i - j) for its
-own key j <= i. Both run without gradients.
+own key j <= i. Both run without gradients (and the kernels refuse
+forward-mode tangents).
 
 A key whose weight is below 2^-150 of the row's largest adds nothing; on a GPU
 its value is then not looked at, so a NaN in it need not show. The kernels

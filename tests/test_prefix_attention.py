@@ -13,6 +13,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from photon_amd.ops.attention import alibi_slopes, reference_attention_fp32
 from photon_amd.ops.prefix_attention import (
@@ -221,6 +222,23 @@ def test_plain_path_on_a_gpu_keeps_bad_values_in_their_sequence(dev):
 @gpu
 def test_gpu_refused_cache_stays(dev):
     refused_cache_stays(dev)
+
+
+@gpu
+@pytest.mark.parametrize("which", range(4))
+def test_forward_mode_is_refused(dev, which):
+    H, D = 2, 64
+    qkv, prefix, slopes = make(dev, 3, 9, H, D)
+    cache, held = torch.zeros(3, 4, 2, H, D, dtype=BF16, device=dev), torch.zeros(3, dtype=torch.int32, device=dev)
+    with fwAD.dual_level():
+        args = [qkv, prefix, slopes, cache]
+        args[which] = fwAD.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError, match="prefix_attention_decode: forward-mode"):
+            prefix_attention_decode(args[0], args[1], H, args[2], args[3], held)
+        assert bool((cache == 0).all())
+        if which < 3:
+            with pytest.raises(NotImplementedError, match="prefix_attention_qkv: forward-mode"):
+                prefix_attention_qkv(args[0], args[1], H, args[2], sequence_starts([3], dev))
 
 
 @gpu
