@@ -10,13 +10,15 @@ where that is below 1; the norm never leaves the device.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import hip_ext, use_hip
 
 
 def tensor_norms(tensors) -> tuple[torch.Tensor, torch.Tensor]:
     """(global L2 norm, [n] L2 norm of each) of fp32 and bf16 tensors on one
-    device, as fp32 tensors there. The tensors stay as they are."""
+    device, as fp32 tensors there. The tensors stay as they are; no derivative
+    passes through."""
     tensors = list(tensors)
     if not tensors:
         return torch.zeros(()), torch.zeros(0)
@@ -47,6 +49,9 @@ def clip_grads_(grads, max_norm: float) -> tuple[torch.Tensor, torch.Tensor]:
     if not torch.is_inference_mode_enabled() and any(g.is_inference() for g in grads):
         raise RuntimeError("clip_grads_: a gradient was made in inference mode "
                            "and cannot be written outside of it")
+    if forward_ad._current_level >= 0 and any(
+            forward_ad.unpack_dual(g).tangent is not None for g in grads):
+        raise NotImplementedError("clip_grads: forward-mode derivatives are not supported")
     total, norms = tensor_norms(grads)
     scale = max_norm / (total + 1e-6)
     if not scale >= 1.0:

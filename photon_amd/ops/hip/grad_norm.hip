@@ -264,6 +264,7 @@ std::vector<torch::Tensor> clip_grads(std::vector<torch::Tensor> gs,
   for (const auto& g : gs) {
     TORCH_CHECK(g.layout() == at::kStrided, "clip_grads: strided tensors only");
     check_writable(g, "clip_grads", "a gradient");
+    check_no_tangent(g, "clip_grads");
     if (g.numel() == 0) continue;
     long span = 1;
     for (int d = 0; d < g.dim(); ++d) {

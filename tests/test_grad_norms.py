@@ -10,6 +10,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from photon_amd.ops.clip import clip_grad_norm_, clip_grads_, tensor_norms
 
@@ -103,6 +104,21 @@ def refused_gradients_stay(dev):
 
 def test_refused_gradients_stay():
     refused_gradients_stay("cpu")
+
+
+def forward_mode_is_refused(dev):
+    """The factor depends on every gradient: a tangent scaled by it, or left
+    as it is, would be wrong."""
+    g, other = torch.full((5,), 2.0, device=dev), torch.full((3,), 2.0, device=dev)
+    with fwAD.dual_level():
+        dual = fwAD.make_dual(g, torch.ones_like(g))
+        with pytest.raises(NotImplementedError, match="clip_grads: forward-mode"):
+            clip_grads_([other, dual], 0.1)
+    assert bool((g == 2.0).all()) and bool((other == 2.0).all())
+
+
+def test_forward_mode_is_refused():
+    forward_mode_is_refused("cpu")
 
 
 def test_optimizer_monitor_matches_the_loop():
@@ -207,6 +223,11 @@ def test_strided_gradients(dev):
 @gpu
 def test_gpu_refused_gradients_stay(dev):
     refused_gradients_stay(dev)
+
+
+@gpu
+def test_gpu_forward_mode_is_refused(dev):
+    forward_mode_is_refused(dev)
 
 
 @gpu
