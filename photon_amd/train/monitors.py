@@ -12,6 +12,7 @@ decoder flops model: 6*N params + causal attention term per token.
 
 from __future__ import annotations
 
+import math
 import time
 from collections import deque
 
@@ -98,10 +99,32 @@ class RuntimeEstimator:
         return {"time/remaining_estimate": remaining * rate}
 
 
+def _norms(tensors: list) -> list[float]:
+    """[global, each]: one sweep and one wait for the strided fp32 and bf16
+    tensors of each device, and a sum of its own for every other tensor."""
+    sweeps: dict = {}
+    rest = []
+    for i, t in enumerate(tensors):
+        swept = (t.layout == torch.strided
+                 and t.dtype in (torch.float32, torch.bfloat16)
+                 and type(t) in (torch.Tensor, torch.nn.Parameter))
+        (sweeps.setdefault(t.device, []) if swept else rest).append(i)
+    if not rest and len(sweeps) <= 1:
+        total, each = tensor_norms(tensors)
+        return torch.cat([total.reshape(1), each]).tolist()
+    each = [0.0] * len(tensors)
+    for at in sweeps.values():
+        for i, norm in zip(at, tensor_norms([tensors[i] for i in at])[1].tolist()):
+            each[i] = norm
+    for i in rest:
+        each[i] = math.sqrt(float(tensors[i].detach().double().square().sum()))
+    return [math.sqrt(math.fsum(n * n for n in each)), *each]
+
+
 class OptimizerMonitor:
     """L2 norms of the first moments and the gradients (reference
     optimizer_monitor): the global ones, and with ``only_global`` False each
-    parameter's too. One sweep over all tensors and one wait for the device."""
+    parameter's too."""
 
     def __init__(self, interval: int | str = 10, only_global: bool = True):
         self.interval = (
@@ -128,8 +151,7 @@ class OptimizerMonitor:
         out = {}
         for key, found in (("optimizer/l2_norm_first_moment", moments),
                            ("optimizer/l2_norm_grad", grads)):
-            total, each = tensor_norms([t for _, t in found.values()])
-            values = torch.cat([total.reshape(1), each]).tolist()
+            values = _norms([t for _, t in found.values()])
             out[key] = values[0]
             if not self.only_global:
                 out.update((f"{key}/{n}", v) for (n, _), v in

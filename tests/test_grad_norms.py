@@ -146,6 +146,41 @@ def test_optimizer_monitor_matches_the_loop():
     assert OptimizerMonitor(interval="10ba").batch_end(tr, 0.0) == {}
 
 
+def monitor_takes_any_tensor(devices):
+    """Half and double gradients and moments, sparse ones, parameters on
+    several devices: each norm within fp32's rounding, as a loop over them gave."""
+    from types import SimpleNamespace
+
+    from photon_amd.train.monitors import OptimizerMonitor
+
+    g = torch.Generator().manual_seed(4)
+    model, opt = torch.nn.Module(), SimpleNamespace(state={}, param_groups=[])
+    dtypes = [F32, torch.float16, BF16, torch.float64]
+    for i in range(9):
+        p = torch.nn.Parameter(torch.randn(7, i + 1, generator=g).to(devices[i % len(devices)], dtypes[i % 4]))
+        p.grad = torch.randn(7, i + 1, generator=g).to(p)
+        opt.state[p] = {"exp_avg": torch.randn(7, i + 1, generator=g).to(p).t()}
+        if i == 8:
+            p.grad = p.grad.to_sparse()
+        opt.param_groups.append({"params": [p]})
+        model.register_parameter(f"p{i}", p)
+    tr = SimpleNamespace(optimizer=opt, model=model, timestamp=SimpleNamespace(batch=20))
+    got = OptimizerMonitor(only_global=False).batch_end(tr, 0.0)
+    for key, pick in (("optimizer/l2_norm_grad", lambda p: p.grad.to_dense()),
+                      ("optimizer/l2_norm_first_moment", lambda p: opt.state[p]["exp_avg"])):
+        each = {n: float(pick(p).detach().double().square().sum()) for n, p in model.named_parameters()}
+        for n, s in each.items():
+            assert abs(got[f"{key}/{n}"] - math.sqrt(s)) <= 2.0**-23 * math.sqrt(s)
+        # each norm is rounded to fp32 before its square joins the others
+        want = math.sqrt(sum(each.values()))
+        assert abs(got[key] - want) <= 2.0**-22 * want
+    assert len(got) == 20
+
+
+def test_optimizer_monitor_takes_any_tensor():
+    monitor_takes_any_tensor(["cpu"])
+
+
 # -- GPU --------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def dev():
@@ -228,6 +263,13 @@ def test_gpu_refused_gradients_stay(dev):
 @gpu
 def test_gpu_forward_mode_is_refused(dev):
     forward_mode_is_refused(dev)
+
+
+@gpu
+def test_gpu_optimizer_monitor_takes_any_tensor(dev):
+    monitor_takes_any_tensor([dev])
+    monitor_takes_any_tensor(["cpu", dev])
+    monitor_takes_any_tensor([dev, dev, "cpu"])
 
 
 @gpu
