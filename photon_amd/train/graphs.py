@@ -17,8 +17,6 @@ Contract:
   path pads nothing and always ticks full microbatches;
 * gradients ACCUMULATE into the captured .grad tensors — callers must zero
   with ``set_to_none=False`` (zero_()), never free them;
-* no loss of an earlier eager pass over the same parameters is alive when the
-  first microbatch is captured;
 * the optimizer step and scheduler run OUTSIDE the graph (dynamic lr);
 * weight VALUES may change between replays (the fed round copies new
   globals into the same parameter tensors — graph-safe).
@@ -53,18 +51,29 @@ class GraphedMicrobatch:
                     out = self.model(self.static_ids, labels=self.static_ids)
                     loss = out["loss"] / self.loss_div
                     loss.backward()
-        # A live eager graph keeps the leaves' accumulation nodes on the
-        # warm-up's stream, and a captured backward must not wait for that one.
         del out, loss
         torch.cuda.current_stream().wait_stream(s)
         self._zero_grads()
+        # A live eager graph (a loss that somebody keeps) holds the parameters'
+        # accumulation nodes on the stream that it ran on, and a captured
+        # backward must not wait for that one. So the capture has leaves of its
+        # own: other nodes over the same memory and the same gradients.
+        params = dict(self.model.named_parameters())
+        leaves = {n: torch.nn.Parameter(p.data, requires_grad=p.requires_grad)
+                  for n, p in params.items()}
+        for n, p in params.items():
+            leaves[n].grad = p.grad
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             with self._autocast():
-                out = self.model(self.static_ids, labels=self.static_ids)
+                out = torch.func.functional_call(
+                    self.model, leaves, (self.static_ids,),
+                    {"labels": self.static_ids})
                 loss = out["loss"] / self.loss_div
                 loss.backward()
             self._static_loss = loss.detach()
+        for n, p in params.items():
+            p.grad = leaves[n].grad
         self._graph = g
 
     def _zero_grads(self):

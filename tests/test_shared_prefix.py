@@ -305,6 +305,42 @@ def test_train_clip_then_score(dev):
 
 
 @gpu
+def test_microbatch_captured_beside_a_live_loss(dev):
+    """A loss of an eager pass over the same parameters is alive while the
+    microbatch is captured and replayed, and is used afterwards. Bounds as in
+    the next test."""
+    from photon_amd.train.graphs import GraphedMicrobatch
+
+    def amp():
+        return torch.autocast("cuda", dtype=torch.bfloat16)
+
+    eager, graphed = (tiny("flash", 256, 4, emb_scale=2.0).train().to(dev) for _ in range(2))
+    ids = torch.randint(0, 300, (2, 64), device=dev)
+
+    def both(f, model):
+        with amp():
+            loss = model(ids, labels=ids)["loss"]
+            f(loss)
+        return loss
+
+    live = both(lambda loss: None, graphed)
+    g = GraphedMicrobatch(graphed, amp, 1.0, 2, 64, dev)
+    loss = float(g.run(ids))
+    both(lambda loss: loss.backward(), eager)
+    held = [p.grad for p in graphed.parameters()]
+    for times in (1, 2, 3):  # replayed once more each, then the live one's backward
+        for a, b in zip(graphed.parameters(), eager.parameters()):
+            assert (a.grad - times * b.grad).norm() <= 2.0**-8 * times * b.grad.norm()
+        if times == 1:
+            assert abs(float(g.run(ids)) - loss) <= 2.0**-8 * loss
+        elif times == 2:
+            with amp():
+                live.backward()
+    assert all(p.grad is h for p, h in zip(graphed.parameters(), held))
+    assert abs(float(live.detach()) - loss) <= 2.0**-8 * loss
+
+
+@gpu
 def test_graphed_microbatch_matches_eager(dev):
     """Lookup and gradient inside the captured training microbatch. Should a
     library product choose another split in a graph, a bf16 value rounds to
