@@ -58,6 +58,7 @@ class SharedPrefix:
         self._held: torch.Tensor | None = None
         self._steps = self._slots = 0
 
+    @torch.no_grad()
     def logits(self, hidden: torch.Tensor) -> torch.Tensor:
         return F.linear(hidden, self.model.transformer.wte.weight)
 

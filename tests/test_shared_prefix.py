@@ -207,6 +207,16 @@ def test_inference_mode():
     inference_mode_matches(tiny(), "cpu")
 
 
+def test_nothing_keeps_a_graph():
+    """Runs without gradients, its logits too, wherever it is called from."""
+    m = tiny()
+    assert m.transformer.wte.weight.requires_grad and torch.is_grad_enabled()
+    shared = SharedPrefix(m, [1, 2, 3])
+    shared.begin(2, 1)
+    outs = [shared.last_hidden, shared.score([[4, 5], [6]]), shared.step(torch.tensor([7, 8]))]
+    assert not any(t.requires_grad for x in outs for t in (x, shared.logits(x)))
+
+
 def test_emb_scale_in_the_model():
     """emb_scale is read from the configuration, survives a resize, and 1.0
     leaves the model as it was."""
