@@ -43,7 +43,7 @@ def embedding(
         raise ValueError(f"embedding: table must be [V, D], got {tuple(table.shape)}")
     y = F.embedding(ids, table)
     if scale != 1.0:
-        y = y.float() * scale
+        y = y.to(torch.promote_types(y.dtype, torch.float32)) * scale
     return y.to(out_dtype)
 
 

@@ -52,6 +52,14 @@ def test_plain_path(table_dtype, out_dtype):
     assert bool(((g.double() - want).abs() <= (terms + 2) * eps * mag + 1e-300).all())
 
 
+def test_plain_path_keeps_64_bits():
+    w = torch.randn(5, 3, dtype=torch.float64, requires_grad=True)
+    ids = torch.tensor([4, 0, 4])
+    y = embedding(ids, w, 1.0 / 3.0)
+    assert y.dtype == torch.float64 and torch.equal(y, w[ids] * (1.0 / 3.0))
+    assert torch.autograd.gradcheck(lambda t: embedding(ids, t, 1.0 / 3.0), (w,))
+
+
 def test_refusals():
     w = torch.randn(4, 8)
     with pytest.raises(TypeError, match="int64 or int32"):
