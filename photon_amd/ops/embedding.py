@@ -31,9 +31,9 @@ def embedding(
     """Rows ``ids`` (int64 or int32, any shape) of ``table`` [V, D] (fp32 or
     bf16), times ``scale``, as ``out_dtype`` (default: the table's).
 
-    Differentiable once in ``table``; on the GPU not in forward mode. An id outside [0, V) raises IndexError
-    on the CPU; on the GPU, where looking would wait for the device, its row
-    is NaN and it has no gradient."""
+    Differentiable once in ``table``; on the GPU not in forward mode. An id
+    outside [0, V) raises IndexError on the CPU; on the GPU, where looking
+    would wait for the device, its row is NaN and it has no gradient."""
     out_dtype = out_dtype or table.dtype
     if use_hip(table):  # checks the same
         return hip_ext().embedding(ids, table, scale, out_dtype)
@@ -41,6 +41,9 @@ def embedding(
         raise TypeError(f"embedding: ids must be int64 or int32, got {ids.dtype}")
     if table.dim() != 2:
         raise ValueError(f"embedding: table must be [V, D], got {tuple(table.shape)}")
+    if table.dtype == torch.bfloat16 and table.requires_grad \
+            and torch.is_grad_enabled():
+        table = table.float()  # torch adds the gradient up in the table's type
     y = F.embedding(ids, table)
     if scale != 1.0:
         y = y.to(torch.promote_types(y.dtype, torch.float32)) * scale

@@ -60,6 +60,24 @@ def test_plain_path_keeps_64_bits():
     assert torch.autograd.gradcheck(lambda t: embedding(ids, t, 1.0 / 3.0), (w,))
 
 
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("scale", [1.0, 0.5])
+def test_plain_gradient_of_a_bf16_table_sums_in_32_bits(scale, out_dtype):
+    """Whole numbers, the sums below 2^24: exact until the one rounding. A sum
+    of 1000 ones that rounds to bf16 at each step stops at 256."""
+    g = torch.Generator().manual_seed(7)
+    ids = torch.randint(0, 4, (4000,), generator=g)
+    ids[:1000] = 3
+    dy = torch.randint(-3, 5, (4000, 6), generator=g).to(out_dtype)
+    dy[ids == 3] = 1.0
+    w = torch.randn(4, 6, generator=g).to(BF16).requires_grad_()
+    y = embedding(ids, w, scale, out_dtype)
+    assert torch.equal(y, (w[ids].float() * scale).to(out_dtype))
+    (got,) = torch.autograd.grad(y, w, dy)
+    want, _, _ = exact_grad(ids, dy, 4, scale)
+    assert torch.equal(got, want.to(BF16)) and float(want[3, 0]) >= 1000 * scale
+
+
 def test_refusals():
     w = torch.randn(4, 8)
     with pytest.raises(TypeError, match="int64 or int32"):
