@@ -236,6 +236,65 @@ def test_emb_scale_in_the_model():
     assert m.transformer.wte.scale == 8.0 and m.transformer.wte(ids).shape == (2, 5, 64)
 
 
+def loud(impl, heads):
+    """A model whose attention is most of what it says: queries, keys and
+    values 5 times the usual, their projection 20 times.
+
+    Two bf16 runs of it: some 24 roundings, each 0.42 * 2^-8 of the hidden
+    state rms, added at random, move a logit of std 0.33 by 0.0027, two runs by
+    0.0038 apart; the logits, up to 1.5, are rounded to 2^-8 in either. The
+    largest of 10^4 is at 4 sigma, 0.015 + 0.008: LOGIT is twice that. A mean
+    cross-entropy of one token, 3 sigma, 0.0114 + 0.0078: CE."""
+    m = tiny(impl, 256, heads)
+    with torch.no_grad():
+        for block in m.transformer.blocks:
+            block.attn.Wqkv.weight.mul_(5.0)
+            block.attn.out_proj.weight.mul_(20.0)
+    return m
+
+
+LOGIT, CE = 0.05, 0.02
+LOUD_PREFIX = [(37 * i) % 300 for i in range(90)]
+
+
+@pytest.mark.parametrize("mistake", ["last key", "no bias", "one sequence"])
+@pytest.mark.parametrize("heads", [4, 2])
+def test_a_mistake_moves_the_loud_model(monkeypatch, heads, mistake):
+    """What the GPU tests of this model allow is far below what a wrong call
+    does to its logits and scores."""
+    from photon_amd.models import shared_prefix
+    from photon_amd.ops.prefix_attention import prefix_attention_decode, prefix_attention_qkv
+
+    def planted(call):
+        def wrong(qkv, prefix, h, slopes, *rest, impl="flash"):
+            if mistake == "last key":
+                prefix = prefix[:-1]
+            elif mistake == "no bias":
+                slopes = slopes * 0.0
+            else:  # all rows of the first sequence, all slots empty
+                rest = (*rest[:-1], rest[-1] * 0)
+            return call(qkv, prefix, h, slopes, *rest, impl=impl)
+        return wrong
+
+    m, tok = loud("torch", heads), ByteTokenizer()
+
+    def outputs():
+        s = SharedPrefix(m, LOUD_PREFIX)
+        s.begin(2, 2)
+        return [s.logits(s.score(SEQS)), *(s.logits(s.step(torch.tensor([i, 7]))) for i in (5, 9))]
+
+    want = outputs()
+    ces = [_continuation_stats(m, tok, c, a, "cpu", 100) for p in PAIRS for c, a in p]
+    monkeypatch.setattr(shared_prefix, "prefix_attention_qkv", planted(prefix_attention_qkv))
+    monkeypatch.setattr(shared_prefix, "prefix_attention_decode", planted(prefix_attention_decode))
+    for a, b in zip(want[::2], outputs()[::2]):  # scores, the second step
+        assert (a - b).abs().max() > 4 * LOGIT
+    if heads == 2:  # slopes of 2^-4 and 2^-8 say little in these short texts
+        return
+    wrong = [x for p in PAIRS for x in _shared_stats(m, tok, p, "cpu", 100)]
+    assert max(abs(a[0] - b[0]) / max(a[1], 1) for a, b in zip(ces, wrong)) > 4 * CE
+
+
 # -- GPU --------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def dev():
@@ -255,6 +314,25 @@ def test_gpu_scores_match_whole_sequences(dev, d, heads, weights):
     else:
         with torch.autocast("cuda", dtype=torch.bfloat16):
             assert_scores(m, prefix, SEQS, 0.1)
+
+
+@gpu
+@pytest.mark.parametrize("heads", [4, 2])
+@pytest.mark.parametrize("weights", ["autocast", "bf16"])
+def test_gpu_scores_of_the_loud_model(dev, heads, weights):
+    m, tok = loud("flash", heads).to(dev), ByteTokenizer()
+    if weights == "bf16":
+        m = m.to(torch.bfloat16)
+    with torch.autocast("cuda", dtype=torch.bfloat16, enabled=weights == "autocast"):
+        assert_scores(m, LOUD_PREFIX, SEQS, LOGIT)
+        for pairs in PAIRS:
+            want = [_continuation_stats(m, tok, c, a, dev, 100) for c, a in pairs]
+            got = _shared_stats(m, tok, pairs, dev, 100)
+            mean, mean2 = ([ce / max(n, 1) for ce, n, _ in s] for s in (want, got))
+            assert [n for _, n, _ in want] == [n for _, n, _ in got]
+            assert all(abs(a - b) <= CE for a, b in zip(mean, mean2))
+            if len(pairs) > 1 and sorted(mean)[1] - min(mean) > 2 * CE:
+                assert mean.index(min(mean)) == mean2.index(min(mean2))
 
 
 @gpu
