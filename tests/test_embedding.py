@@ -186,6 +186,27 @@ def test_many_ids_over_all_sort_blocks(dev):
 
 
 @gpu
+@pytest.mark.parametrize("table_dtype,dy_dtype", [(F32, BF16), (F32, F32), (BF16, BF16)])
+@pytest.mark.parametrize("n,V,D,top", [
+    (200_003, 50368, 16, 0.5), (40000, 512, 100, 0.3), (1_000_003, 300, 4, 0.99),
+    (65536, 50368, 768, 0.0), (16384, 70000, 40, 0.9), (270_000, 2, 1, 0.5),
+    (1_100_000, 50257, 8, 1.0),
+])
+def test_frequent_tokens_are_summed_exactly(dev, table_dtype, dy_dtype, n, V, D, top):
+    """Whole numbers up to 8 and a scale of a power of two: every fp32 sum is
+    below 2^24 and exact in any order, so a partial sum that is lost or counted
+    twice shows however many terms there are. A bf16 table rounds once."""
+    w, ids, _ = make(dev, n, V, D, table_dtype, dy_dtype)
+    g = torch.Generator(device=dev).manual_seed(n)
+    ids[torch.rand(n, generator=g, device=dev) < top] = V - 1
+    dy = torch.randint(-8, 9, (n, D), generator=g, device=dev).to(dy_dtype)
+    (got,) = torch.autograd.grad(embedding(ids, w, 0.5, dy_dtype), w, dy)
+    want, mag, _ = exact_grad(ids, dy, V, 0.5)
+    assert float(mag.max()) < 2**23  # times the scale
+    assert torch.equal(got.cpu(), want.to(table_dtype))
+
+
+@gpu
 @pytest.mark.parametrize("n", [4096, 4097, 16383, 16384, 16385])
 @pytest.mark.parametrize("V", [200, 300, 70000, 20_000_000])
 def test_both_sorts_over_one_to_four_passes(dev, n, V):
