@@ -27,9 +27,6 @@ void adopt_step(std::vector<torch::Tensor> ps, std::vector<torch::Tensor> gs,
                 double lr, double b1, double b2, double eps, double wd,
                 double clip, long step,
                 std::vector<torch::Tensor> masters);
-torch::Tensor multi_tensor_l2norm(std::vector<torch::Tensor> gs);
-void multi_tensor_scale_clip(std::vector<torch::Tensor> gs,
-                             torch::Tensor total_norm, double max_norm);
 std::vector<torch::Tensor> attn_fwd_qkv(torch::Tensor qkv, long H,
                                         torch::Tensor slopes, bool causal);
 torch::Tensor attn_bwd_qkv(torch::Tensor dout, torch::Tensor qkv, long H,
@@ -84,8 +81,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "fused CE loss + in-place softmax gradient");
   m.def("adamw_step", &adamw_step, "fused multi-tensor AdamW step");
   m.def("adopt_step", &adopt_step, "fused multi-tensor ADOPT step");
-  m.def("multi_tensor_l2norm", &multi_tensor_l2norm);
-  m.def("multi_tensor_scale_clip", &multi_tensor_scale_clip);
   m.def("attn_fwd", &attn_fwd_launch, "flash attention forward (ALiBi fused)");
   m.def("attn_bwd", &attn_bwd_launch, "flash attention backward");
   m.def("lt_linear_fwd", &lt_linear_fwd,

@@ -1,4 +1,4 @@
-// Fused multi-tensor AdamW / ADOPT / grad-clip kernels for CDNA4.
+// Fused multi-tensor AdamW / ADOPT kernels for CDNA4.
 //
 // Replaces torch's _fused_adamw multi-tensor-apply + the reference "adopt"
 // optimizer. Tensors are batched into a struct
@@ -87,59 +87,6 @@ __global__ void adopt_kernel(TensorBatch<T> batch, float lr, float b1,
   }
 }
 
-// -- multi-tensor L2 norm (two-stage, deterministic) ------------------------
-template <typename T, int BLOCK>
-__global__ void l2norm_partial_kernel(TensorBatch<T> batch,
-                                      float* __restrict__ partials) {
-  __shared__ float scratch[BLOCK / WAVE];
-  const int t = blockIdx.x % batch.count;
-  const int nb = (gridDim.x + batch.count - 1 - t) / batch.count;
-  const int bi = blockIdx.x / batch.count;
-  const T* g = batch.g[t];
-  const long n = batch.n[t];
-  float s = 0.f;
-  for (long i = (long)(bi * BLOCK + threadIdx.x); i < n; i += (long)nb * BLOCK) {
-    float v = load_f32<T>(g, i);
-    s += v * v;
-  }
-  s = block_reduce_sum(s, scratch);
-  if (threadIdx.x == 0) partials[blockIdx.x] = s;
-}
-
-__global__ void l2norm_finish_kernel(const float* __restrict__ partials,
-                                     int n, float* __restrict__ out,
-                                     int accumulate) {
-  __shared__ float scratch[256 / WAVE];
-  float s = 0.f;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) s += partials[i];
-  s = block_reduce_sum(s, scratch);
-  if (threadIdx.x == 0) {
-    if (accumulate)
-      out[0] += s;
-    else
-      out[0] = s;
-  }
-}
-
-// scale grads by max_norm/total_norm if above threshold; norm read on
-// device (no host sync).
-template <typename T, int BLOCK>
-__global__ void scale_clip_kernel(TensorBatch<T> batch,
-                                  const float* __restrict__ total_norm,
-                                  float max_norm) {
-  const float total = total_norm[0];
-  const float scale = max_norm / (total + 1e-6f);
-  if (scale >= 1.f) return;
-  const int t = blockIdx.x % batch.count;
-  const int nb = (gridDim.x + batch.count - 1 - t) / batch.count;
-  const int bi = blockIdx.x / batch.count;
-  T* g = batch.g[t];
-  const long n = batch.n[t];
-  for (long i = (long)(bi * BLOCK + threadIdx.x); i < n; i += (long)nb * BLOCK) {
-    store_f32<T>(g, i, load_f32<T>(g, i) * scale);
-  }
-}
-
 // ---------------------------------------------------------------------------
 // Host launchers
 // ---------------------------------------------------------------------------
@@ -200,44 +147,6 @@ void adopt_step(std::vector<torch::Tensor> ps, std::vector<torch::Tensor> gs,
                          dim3(OPT_BLOCK), 0, cur_stream(), batch, (float)lr,
                          (float)b1, (float)b2, (float)eps, (float)wd,
                          (float)clip, (int)step);
-    });
-  }
-}
-
-torch::Tensor multi_tensor_l2norm(std::vector<torch::Tensor> gs) {
-  TORCH_CHECK(!gs.empty(), "multi_tensor_l2norm: empty grad list");
-  const int GRID = 512;
-  const size_t nbatches = (gs.size() + MT_CHUNK - 1) / MT_CHUNK;
-  auto partials = torch::zeros({(long)(nbatches * GRID)},
-                               gs[0].options().dtype(at::kFloat));
-  for (size_t b = 0; b < nbatches; ++b) {
-    size_t s = b * MT_CHUNK;
-    size_t c = std::min((size_t)MT_CHUNK, gs.size() - s);
-    DISPATCH_DTYPE(gs[s], "multi_tensor_l2norm", {
-      auto batch = make_batch<scalar_t>(nullptr, gs, nullptr, nullptr, s, c);
-      hipLaunchKernelGGL((l2norm_partial_kernel<scalar_t, OPT_BLOCK>),
-                         dim3(GRID), dim3(OPT_BLOCK), 0, cur_stream(), batch,
-                         partials.data_ptr<float>() + b * GRID);
-    });
-  }
-  auto total_sq = torch::empty({1}, partials.options());
-  hipLaunchKernelGGL(l2norm_finish_kernel, dim3(1), dim3(256), 0, cur_stream(),
-                     partials.data_ptr<float>(), (int)(nbatches * GRID),
-                     total_sq.data_ptr<float>(), 0);
-  return total_sq.sqrt_().squeeze(0);
-}
-
-void multi_tensor_scale_clip(std::vector<torch::Tensor> gs,
-                             torch::Tensor total_norm, double max_norm) {
-  const int GRID = 1024;
-  auto norm = total_norm.reshape({1}).contiguous();
-  for (size_t s = 0; s < gs.size(); s += MT_CHUNK) {
-    size_t c = std::min((size_t)MT_CHUNK, gs.size() - s);
-    DISPATCH_DTYPE(gs[s], "multi_tensor_scale_clip", {
-      auto batch = make_batch<scalar_t>(nullptr, gs, nullptr, nullptr, s, c);
-      hipLaunchKernelGGL((scale_clip_kernel<scalar_t, OPT_BLOCK>), dim3(GRID),
-                         dim3(OPT_BLOCK), 0, cur_stream(), batch,
-                         norm.data_ptr<float>(), (float)max_norm);
     });
   }
 }
