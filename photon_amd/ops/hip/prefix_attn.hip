@@ -20,9 +20,9 @@ struct Cut {
 };
 
 template <int D>
-using FewRows = Shape<D, 1, 4, 2>;
+using FewRows = Shape<D, 1, 4>;
 template <int D>
-using ManyRows = Shape<D, 4, 1, 2>;
+using ManyRows = Shape<D, 4, 1>;
 // Few rows are 128 items of 32 rows at most: half the chip, so that the keys
 // can be split at least once more. 16 heads of 128 over 1507 keys, 160 rows (80
 // items): 17 us, and 25 with tiles of 128 rows; 32 heads over 3900 keys, 160

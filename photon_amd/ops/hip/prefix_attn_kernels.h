@@ -42,11 +42,11 @@ namespace photon_hip {
 
 // A workgroup is NW x KW waves: NW of 32 query rows each that share their key
 // tiles (64 keys), or, where there are few rows, KW that take every KW-th key
-// tile (32 keys) of the same rows and are joined at the end. BUFS tiles are in
-// LDS or on their way for each.
-template <int D_, int NW_, int KW_, int BUFS_>
+// tile (32 keys) of the same rows and are joined at the end. For each, one tile
+// is in LDS and the next on its way.
+template <int D_, int NW_, int KW_>
 struct Shape {
-  static constexpr int D = D_, NW = NW_, KW = KW_, BUFS = BUFS_;
+  static constexpr int D = D_, NW = NW_, KW = KW_;
   static constexpr int SUBS = KW == 1 ? 2 : 1;  // subtiles of 32 keys
   static constexpr int KEYS = 32 * SUBS;
   static constexpr int IMG = KEYS * D * 2;      // bytes of a [KEYS][D] image
@@ -54,7 +54,7 @@ struct Shape {
   static constexpr int ROWS = 32 * NW;
   // LDS: the images (or, at the end, the waves' fp32 rows), then each wave's
   // maxima and sums; a word a wave for the search of bad values
-  static constexpr int IMAGES = KW * BUFS * 2 * IMG;
+  static constexpr int IMAGES = KW * 2 * 2 * IMG;
   static constexpr int FP32_ROWS = NW * KW * 32 * D * 4;
   static constexpr int STATS = IMAGES > FP32_ROWS ? IMAGES : FP32_ROWS;
   static constexpr int BYTES = STATS + NW * KW * 32 * 8;
@@ -87,12 +87,6 @@ DEV_INLINE void copy16_to_lds(desc_t desc, unsigned lds, int offset) {
       :
       : "s"(lds), "v"(offset), "s"(desc)
       : "memory", "m0");
-}
-
-// Until at most N of this wave's copies are on their way (in order).
-template <int N>
-DEV_INLINE void vm_wait() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 // Until this wave's LDS accesses are done.
@@ -205,10 +199,10 @@ __global__ __launch_bounds__(S::THREADS, S::D == 64 ? 3 : 2) void prefix_attn_ke
     float* __restrict__ part_o, float* __restrict__ part_ml, int T, int P,
     int H, int first_split, int rest, int splits) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int D = S::D, NW = S::NW, KW = S::KW, BUFS = S::BUFS;
+  constexpr int D = S::D, NW = S::NW, KW = S::KW;
   constexpr int SUBS = S::SUBS, KEYS = S::KEYS, IMG = S::IMG;
   constexpr bool D64 = D == 64;
-  constexpr bool STOPS = KW == 1 && BUFS == 2 && !DECODE;
+  constexpr bool STOPS = KW == 1 && !DECODE;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -275,9 +269,9 @@ __global__ __launch_bounds__(S::THREADS, S::D == 64 ? 3 : 2) void prefix_attn_ke
     dma_col[i] =
         (dest ^ (int)(swz_field((unsigned)r & 15u, D64) << 4)) % (D * 2);
   }
-  char* const images = smem + kw * (BUFS * 2 * IMG);
+  char* const images = smem + kw * (2 * 2 * IMG);
   const unsigned wave_win = __builtin_amdgcn_readfirstlane(
-      lds_base(smem) + kw * (BUFS * 2 * IMG) + rw * (NWIN * 1024));
+      lds_base(smem) + kw * (2 * 2 * IMG) + rw * (NWIN * 1024));
   auto stage = [&](int t, int b) {
     const bool pre = t < n_pre;
     const long rs = pre ? p_rs : q_rs;
@@ -303,9 +297,7 @@ __global__ __launch_bounds__(S::THREADS, S::D == 64 ? 3 : 2) void prefix_attn_ke
   // leave before anything else is loaded.
   const int last = t1 - 1 - kw;
   auto first_copies = [&]() {
-#pragma unroll
-    for (int i = 0; i < BUFS - 1; ++i)
-      if (last - i * KW >= t0) stage(last - i * KW, i);
+    if (last >= t0) stage(last, 0);
   };
   if constexpr (KW > 1) first_copies();
 
@@ -492,15 +484,10 @@ __global__ __launch_bounds__(S::THREADS, S::D == 64 ? 3 : 2) void prefix_attn_ke
   // waits for the query's inside the loop, and with them for the next tile.
   __builtin_amdgcn_s_waitcnt(0x0F70);
   if constexpr (KW == 1) first_copies();
-  int b = BUFS - 1;
+  int b = 1;
   for (int t = last; t >= t0; t -= KW) {
-    const int old = b;  // the buffer of the tile before
-    b = b == BUFS - 1 ? 0 : b + 1;
-    // the copies of the BUFS - 2 tiles behind t may still be on their way
-    if (t - (BUFS - 2) * KW >= t0)
-      vm_wait<(BUFS - 2) * 2 * NWIN < 63 ? (BUFS - 2) * 2 * NWIN : 63>();
-    else
-      vm_wait0();
+    b ^= 1;
+    vm_wait0();
     // tile t is there, and the reads of the one before are done
     const bool look = STOPS && norms != nullptr && (t & 3) == 0 && t < n_pre;
     int* const done = bad_words + NW;  // read long before the next is written
@@ -520,7 +507,7 @@ __global__ __launch_bounds__(S::THREADS, S::D == 64 ? 3 : 2) void prefix_attn_ke
       for (int w = 0; w < NW; ++w) all &= done[w] != 0;
       if (all) break;  // nothing is on its way
     }
-    if (t - (BUFS - 1) * KW >= t0) stage(t - (BUFS - 1) * KW, old);
+    if (t - KW >= t0) stage(t - KW, b ^ 1);
     const bool pre = t < n_pre;
     const int kv0 = pre ? t * KEYS : lo + (t - n_pre) * KEYS;
     const bool masked = !pre || (t + 1) * KEYS > P;
