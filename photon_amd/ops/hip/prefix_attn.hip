@@ -38,7 +38,9 @@ constexpr long FEW_ITEMS = 128;
 // 10 us: 20 rows of 12 heads of 64 over 701 keys take 8.7 us whole and 10.0 in
 // two, 96 rows of 16 heads of 128 over 1507 keys 20.7 whole and 15.4 in four.
 // `always` (the decode form, which joins anyway): every item leaves partial
-// rows; one sequence over 701 keys takes 12.0 us whole and 10.7 in two.
+// rows. 64 sequences of 12 heads of 64 over 2000 keys take 18.4 us with 128
+// keys a split at least, 13.7 with 256 and 13.4 with 384; 16 sequences of 32
+// heads of 128 over 700 keys 14.0, 13.6 and 15.8.
 Cut cut(long T, int H, int D, long keys, bool always) {
   Cut c;
   c.few = (T + FewRows<64>::ROWS - 1) / FewRows<64>::ROWS * H <= FEW_ITEMS;
