@@ -259,7 +259,8 @@ std::vector<torch::Tensor> clip_grads(std::vector<torch::Tensor> gs,
                                       double max_norm) {
   TORCH_CHECK(!gs.empty(), "clip_grads: empty list of tensors");
   const c10::DeviceGuard guard(gs[0].device());
-  // A gradient that is there twice would be scaled twice, or half of it.
+  // A gradient that is there twice would be counted and scaled twice, or half
+  // of it. Of a strided one, whose gaps may hold others, the first element.
   std::vector<std::pair<uintptr_t, uintptr_t>> spans;
   for (const auto& g : gs) {
     TORCH_CHECK(g.layout() == at::kStrided, "clip_grads: strided tensors only");
@@ -274,8 +275,8 @@ std::vector<torch::Tensor> clip_grads(std::vector<torch::Tensor> gs,
                   "clip_grads: a gradient shares elements with itself");
     }
     const auto p = (uintptr_t)g.data_ptr();
-    if (g.is_non_overlapping_and_dense())
-      spans.emplace_back(p, p + span * g.element_size());
+    if (!g.is_non_overlapping_and_dense()) span = 1;
+    spans.emplace_back(p, p + span * g.element_size());
   }
   std::sort(spans.begin(), spans.end());
   for (size_t i = 1; i < spans.size(); ++i)

@@ -273,6 +273,22 @@ def test_gpu_optimizer_monitor_takes_any_tensor(dev):
 
 
 @gpu
+def test_strided_gradients_that_share_memory(dev):
+    """Named twice, from one element on, or out of a dense one; views that
+    only lie between each other are taken (test_strided_gradients)."""
+    a = torch.randn(8, 12, device=dev)
+    old = a.clone()
+    for bad in ([a[:, ::2], a[:, ::2]], [a[:, ::2], a[:, ::3]], [a, a[:, 1::2]], [a[2:, 3::4], a]):
+        with pytest.raises(RuntimeError, match="share memory"):
+            clip_grads_(bad, 0.1)
+        assert torch.equal(a, old)
+    parts = [a[:, 1::2], a[0, 4:5], a[:, 2:4:2]]
+    before = [g.clone() for g in parts]
+    total, norms = clip_grads_(parts, 0.5)
+    assert_clipped(parts, before, total, norms, 0.5)
+
+
+@gpu
 def test_gpu_refusals(dev):
     g = torch.randn(100, device=dev)
     for bad, match in (([g, g], "share memory"), ([g[:60], g[50:]], "share memory"),
