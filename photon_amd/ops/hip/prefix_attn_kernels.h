@@ -25,7 +25,7 @@
 // loaded (Cauchy and Schwarz: q . k <= |q| max |k|, see key_norms_kernel).
 //
 // Measured on an MI355X. Many rows (4416 over 3901 shared keys, 32 heads of
-// 128): 232 us, of which 8 go to the keys' lengths and 8 to the join; 290 GFLOP
+// 128): 234 us, of which 8 go to the keys' lengths and 8 to the join; 290 GFLOP
 // by the formula, 174 computed. Of the SIMDs' cycles matrix instructions take
 // 32% and vector instructions 38% with little overlap, LDS accesses 22% of the
 // CUs'; the rest is waiting, at 1.6 waves a SIMD of 2. Few rows (93 over 1507, 16
