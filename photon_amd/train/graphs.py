@@ -57,8 +57,10 @@ class GraphedMicrobatch:
         # A live eager graph (a loss that somebody keeps) holds the parameters'
         # accumulation nodes on the stream that it ran on, and a captured
         # backward must not wait for that one. So the capture has leaves of its
-        # own: other nodes over the same memory and the same gradients.
-        params = dict(self.model.named_parameters())
+        # own: other nodes over the same memory and the same gradients. But for
+        # parameters with hooks, which belong to them and are captured too.
+        params = {n: p for n, p in self.model.named_parameters()
+                  if not (p._backward_hooks or p._post_accumulate_grad_hooks)}
         leaves = {n: torch.nn.Parameter(p.data, requires_grad=p.requires_grad)
                   for n, p in params.items()}
         for n, p in params.items():
@@ -73,7 +75,8 @@ class GraphedMicrobatch:
                 loss.backward()
             self._static_loss = loss.detach()
         for n, p in params.items():
-            p.grad = leaves[n].grad
+            if p.grad is None:
+                p.grad = leaves[n].grad
         self._graph = g
 
     def _zero_grads(self):

@@ -429,6 +429,34 @@ def test_microbatch_captured_beside_a_live_loss(dev):
 
 
 @gpu
+def test_hooks_on_parameters_are_captured(dev):
+    """Hooks that double a gradient, on a matrix and, behind the accumulation,
+    on a vector: in every replay, as in an eager pass."""
+    from photon_amd.train.graphs import GraphedMicrobatch
+
+    def amp():
+        return torch.autocast("cuda", dtype=torch.bfloat16)
+
+    def double(p):
+        p.grad.mul_(2.0)
+
+    eager, graphed = (tiny("flash", 256, 4).train().to(dev) for _ in range(2))
+    for m in (eager, graphed):
+        m.transformer.blocks[0].attn.Wqkv.weight.register_hook(lambda g: g * 2.0)
+        m.transformer.norm_f.weight.register_post_accumulate_grad_hook(double)
+    ids = torch.randint(0, 300, (2, 64), device=dev)
+    g = GraphedMicrobatch(graphed, amp, 1.0, 2, 64, dev)
+    with amp():
+        eager(ids, labels=ids)["loss"].backward()
+    for i in range(3):
+        if i:
+            g._zero_grads()
+        g.run(ids)
+        for a, b in zip(graphed.parameters(), eager.parameters()):
+            assert (a.grad - b.grad).norm() <= 2.0**-8 * b.grad.norm()
+
+
+@gpu
 def test_graphed_microbatch_matches_eager(dev):
     """Lookup and gradient inside the captured training microbatch. Should a
     library product choose another split in a graph, a bf16 value rounds to
